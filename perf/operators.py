@@ -187,7 +187,7 @@ def _prepare_prefix(case, seed, g):
                 pool[to, :p % bs] = pool[int(table[firsts[i], p // bs]), :p % bs]
     q = _randn((rows, 1, case["hq"], HEAD_DIM), g)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
-    return {"op": "prefix", "q": q, "k": k, "v": v, "table": table.cuda(), "lens": i32(lens), "prefix_lens": i32(shared),
+    return {"op": "prefix", "q": q, "k": k, "v": v, "table": table.cuda(), "lens": i32(lens), "prefix_lens": i32(prefixes),
             "cu_rows": i32(firsts + [sum(sizes)]), "most_rows": max(sizes), "most_prefix": max(prefixes),
             "most_own": max(1, max(suffix))}
 
@@ -235,10 +235,10 @@ def _plain_copy(pool, src, dst, tokens):
 
 def _plain_prefix(st):
     """Scores of the prefix keys once for all rows of a group, of each row's own keys by itself, one softmax over both."""
-    q, k, v, table, lens, shared = (st[x] for x in ("q", "k", "v", "table", "lens", "prefix_lens"))
+    q, k, v, table, lens, prefix = (st[x] for x in ("q", "k", "v", "table", "lens", "prefix_lens"))
     cu, bs, (B, _, hq, D), hkv = st["cu_rows"].long(), st["k"].shape[1], q.shape, st["k"].shape[2]
     grp, scale, inf = hq // hkv, D ** -0.5, float("inf")
-    lens, shared, dev = lens.long(), shared.long(), q.device
+    lens, prefix, dev = lens.long(), prefix.long(), q.device
     qh = q[:, 0].float().view(B, hkv, grp, D) * scale
 
     # rows of the groups, padded to the largest group; a row of padding stands for row B, which is dropped
@@ -246,6 +246,9 @@ def _plain_prefix(st):
     rows = torch.where(rows < cu[1:, None], rows, B)
     G, R = rows.shape
     safe = rows.clamp(max=B - 1)
+    shared = torch.zeros(B + 1, dtype=torch.long, device=dev)
+    shared[rows] = prefix[:, None].expand(G, R)
+    shared = shared[:B]
     j = torch.arange(st["most_prefix"], device=dev)
     page = table[cu[:-1].clamp(max=B - 1)][:, (j // bs).clamp(max=table.shape[1] - 1)].long()
     kp, vp = (x[page, j % bs].float().permute(0, 2, 1, 3) for x in (k, v))                 # [G, hkv, P, D]
