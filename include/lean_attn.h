@@ -54,6 +54,8 @@ typedef enum {
 #define LA_DEVERR_SEQLEN 3         /* a sequence needs more blocks than max_blocks_per_seq */
 #define LA_DEVERR_ROPE_POS 4       /* a position is outside the rope table */
 #define LA_DEVERR_SMEM_ALIGN 5     /* dynamic shared memory base not 1024-byte aligned (kernel returned) */
+#define LA_DEVERR_BLOCK_PAIR 6     /* a copy's destination is another copy's source or destination */
+#define LA_DEVERR_PREFIX 7         /* prefix groups that are not ascending runs of the batch's rows */
 
 int la_version(void);
 const char* la_status_string(int status);
@@ -268,6 +270,83 @@ int la_paged_decode_noalloc(
     void* out, int64_t out_batch_stride, int64_t out_head_stride,
     float* softmax_lse,
     int* dev_error, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged GQA decode for a batch whose rows share long prefixes.
+ *
+ * The same result as la_paged_decode on the same arguments, with the keys of
+ * a shared prefix read once for all the rows that share it. Rows
+ * cu_prefix_rows[g] .. cu_prefix_rows[g+1]-1 (int32 [num_groups + 1], not
+ * decreasing, within 0..batch, else LA_DEVERR_PREFIX) form group g: their
+ * block tables name the same pages for keys 0..prefix_lens[g]-1 (int32
+ * [num_groups]), and those are read through the table of the group's first
+ * row. Only whole pages are taken as shared: prefix_lens[g] is rounded down to
+ * a multiple of block_size, and keys behind that are read through each row's
+ * own table. A row whose cache_seqlens ends before the shared pages do reads
+ * all its keys by itself, and so do rows in no group. Groups may be empty.
+ * Nothing about groups or lengths is read on the host, so one captured graph
+ * serves every division of the batch into at most num_groups groups.
+ * The reference has no counterpart (its requests never share blocks).
+ * Shapes and limits are la_paged_decode's. workspace: at least
+ * la_paged_decode_shared_prefix_workspace_size() bytes, 256-byte aligned;
+ * calls that may overlap on the GPU need one each.
+ * ------------------------------------------------------------------------ */
+int la_paged_decode_shared_prefix_workspace_size(int device, int batch, int num_groups, int num_q_heads,
+                                                 int num_kv_heads, int head_dim, size_t* bytes);
+
+int la_paged_decode_shared_prefix(
+    const void* q, int64_t q_batch_stride, int64_t q_head_stride,
+    const void* k_cache, const void* v_cache,
+    int64_t kv_block_stride, int64_t kv_token_stride, int64_t kv_head_stride,
+    int64_t num_blocks, int block_size,
+    const int32_t* block_table, int64_t bt_seq_stride, int max_blocks_per_seq,
+    const int32_t* cache_seqlens,
+    const int32_t* prefix_lens, const int32_t* cu_prefix_rows, int num_groups,
+    int batch, int num_q_heads, int num_kv_heads, int head_dim,
+    float softmax_scale,
+    void* out, int64_t out_batch_stride, int64_t out_head_stride,
+    float* softmax_lse,
+    void* workspace, size_t workspace_bytes,
+    int* dev_error, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Pages of the cache, copied and moved on the device.
+ *
+ * k_pool / v_pool: [num_layers, num_blocks, block_size, num_kv_heads,
+ * head_dim] of element_size (1, 2 or 4) bytes, head_dim contiguous, the same
+ * strides (in elements) for both; every stride and head_dim a multiple of 16
+ * bytes. src_blocks / dst_blocks: int32 [num_pairs] on the device.
+ *
+ * la_copy_blocks copies tokens 0..num_tokens[i]-1 (num_tokens NULL: the whole
+ * page) of page src_blocks[i] to page dst_blocks[i] in every layer, K and V:
+ * the copy a forked sequence takes of its last, partly filled page. One page
+ * may be the source of several copies. The reference never shares a block
+ * (leaninfer/engine/cache_manager.py:13-42), so it has no counterpart.
+ *
+ * la_move_blocks copies whole pages and replaces every entry src_blocks[i] of
+ * block_table (int32 [batch, max_blocks_per_seq]) by dst_blocks[i]: a
+ * compaction of the pool.
+ *
+ * The copies run in no particular order. One whose destination is another's
+ * source, or the destination of one before it, is skipped and reported
+ * (LA_DEVERR_BLOCK_PAIR), as are ids outside the pool (LA_DEVERR_BLOCK_ID) and
+ * token counts outside 0..block_size (LA_DEVERR_SEQLEN); a page copied to
+ * itself is left as it is. Table entries of a skipped move stay.
+ * ------------------------------------------------------------------------ */
+int la_copy_blocks(void* k_pool, void* v_pool,
+                   int64_t layer_stride, int64_t block_stride, int64_t token_stride, int64_t head_stride,
+                   int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
+                   int element_size,
+                   const int32_t* src_blocks, const int32_t* dst_blocks, const int32_t* num_tokens, int num_pairs,
+                   int* dev_error, cudaStream_t stream);
+
+int la_move_blocks(void* k_pool, void* v_pool,
+                   int64_t layer_stride, int64_t block_stride, int64_t token_stride, int64_t head_stride,
+                   int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
+                   int element_size,
+                   const int32_t* src_blocks, const int32_t* dst_blocks, int num_pairs,
+                   int32_t* block_table, int64_t bt_seq_stride, int batch, int max_blocks_per_seq,
+                   int* dev_error, cudaStream_t stream);
 
 /* ------------------------------------------------------------------------
  * (c) Causal varlen prefill attention on tcgen05 / TMEM.

@@ -7,6 +7,10 @@ Public API (the drop-ins for the reference's attention path):
   qk_norm_rope_paged_write    fused QK-RMSNorm + RoPE + paged KV write (kernel a)
   paged_kv_write              plain paged KV write (BlockCache.write)
   BlockCache, BlockAllocator  the engine's pool layout and allocator
+and, beyond the reference, for requests that share a prompt:
+  flash_attn_with_shared_prefix  decode that reads a shared prefix once
+  copy_blocks, move_blocks    pages of the cache copied (fork) and moved (compaction)
+  shared_prefix_groups        the groups of rows that share blocks
 The kernels live in _lib/liblean_attn.so (C ABI: include/lean_attn.h).
 """
 from .flash_attn_interface import (  # noqa: F401
@@ -14,12 +18,20 @@ from .flash_attn_interface import (  # noqa: F401
     ensure_init,
     flash_attn_varlen_func,
     flash_attn_with_kvcache,
+    flash_attn_with_shared_prefix,
     paged_kv_write,
     qk_norm_rope_paged_write,
     rope_tables,
     scaled_dot_product_attention,
 )
-from .cache import BlockAllocator, BlockCache, blocks_for  # noqa: F401
+from .cache import (  # noqa: F401
+    BlockAllocator,
+    BlockCache,
+    blocks_for,
+    copy_blocks,
+    move_blocks,
+    shared_prefix_groups,
+)
 
 __all__ = [
     "flash_attn_with_kvcache",
@@ -33,4 +45,8 @@ __all__ = [
     "BlockCache",
     "BlockAllocator",
     "blocks_for",
+    "flash_attn_with_shared_prefix",
+    "copy_blocks",
+    "move_blocks",
+    "shared_prefix_groups",
 ]

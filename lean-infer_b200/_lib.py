@@ -20,6 +20,8 @@ DEVERR_NAMES = {
     3: "sequence longer than its block table",
     4: "position outside the rope table",
     5: "shared memory base misaligned",
+    6: "a copy's destination is another copy's source or destination",
+    7: "prefix groups are not ascending runs of the batch's rows",
 }
 
 
@@ -103,6 +105,37 @@ _SIGNATURES = {
         c_void_p, c_int64, c_int64,
         c_int, c_int,
         c_void_p, c_size_t,
+        c_void_p, c_void_p,
+    ],
+    "la_paged_decode_shared_prefix_workspace_size": [c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_size_t)],
+    "la_paged_decode_shared_prefix": [
+        c_void_p, c_int64, c_int64,
+        c_void_p, c_void_p,
+        c_int64, c_int64, c_int64,
+        c_int64, c_int,
+        c_void_p, c_int64, c_int,
+        c_void_p,
+        c_void_p, c_void_p, c_int,
+        c_int, c_int, c_int, c_int,
+        c_float,
+        c_void_p, c_int64, c_int64,
+        c_void_p,
+        c_void_p, c_size_t,
+        c_void_p, c_void_p,
+    ],
+    "la_copy_blocks": [
+        c_void_p, c_void_p,
+        c_int64, c_int64, c_int64, c_int64,
+        c_int, c_int64, c_int, c_int, c_int, c_int,
+        c_void_p, c_void_p, c_void_p, c_int,
+        c_void_p, c_void_p,
+    ],
+    "la_move_blocks": [
+        c_void_p, c_void_p,
+        c_int64, c_int64, c_int64, c_int64,
+        c_int, c_int64, c_int, c_int, c_int, c_int,
+        c_void_p, c_void_p, c_int,
+        c_void_p, c_int64, c_int, c_int,
         c_void_p, c_void_p,
     ],
     "la_p2p_barrier": [c_void_p, c_int, c_int, c_void_p, c_void_p],

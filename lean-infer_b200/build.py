@@ -18,7 +18,8 @@ INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "liblean_attn.so"
 
-SOURCES = ["la_host.cu", "la_pre_attn.cu", "la_decode.cu", "la_decode_noalloc.cu", "la_prefill.cu", "la_p2p.cu", "la_elementwise.cu", "la_oproj.cu"]
+SOURCES = ["la_host.cu", "la_pre_attn.cu", "la_decode.cu", "la_decode_noalloc.cu", "la_prefill.cu", "la_p2p.cu", "la_elementwise.cu", "la_oproj.cu",
+           "la_prefix.cu", "la_pages.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -9,14 +9,24 @@ Mirrors leaninfer/engine/cache_manager.py:
     scatters k, v [B, Hkv, q_len, D] to block_table[b, col // BS], col % BS,
     col = pos[b] + t. Here write() runs the paged-write kernel instead of
     torch advanced indexing; the result is bit-identical (a copy).
+
+Beyond the reference, whose requests never share a block, blocks may have
+several holders: BlockCache.fork lets sequences share the whole blocks of a
+common prefix (flash_attn_with_shared_prefix reads those once for all of
+them), release gives a block back when its last holder does, and
+BlockCache.compact moves the used blocks to the lowest ids. copy_blocks and
+move_blocks are the device side.
 """
 from __future__ import annotations
 
+import ctypes
 from collections import deque
+from typing import Optional, Sequence
 
 import torch
 
-from .flash_attn_interface import paged_kv_write
+from . import _lib
+from .flash_attn_interface import (_check, _device_index, _ptr, _stream, ensure_init, error_word, paged_kv_write)
 
 
 def blocks_for(n_tokens: int, block_size: int) -> int:
@@ -33,10 +43,13 @@ class InsufficientBlocksError(RuntimeError, AssertionError):
 
 
 class BlockAllocator:
-    """FIFO free list of physical block ids; block 0 is reserved as trash."""
+    """FIFO free list of physical block ids; block 0 is reserved as trash.
+    A block may have several holders (fork); it returns to the free list when
+    the last one releases it."""
 
     def __init__(self, num_blocks: int) -> None:
         self.free: deque[int] = deque(range(1, num_blocks))
+        self._holders: dict[int, int] = {}  # blocks handed out
 
     @property
     def num_free(self) -> int:
@@ -45,10 +58,145 @@ class BlockAllocator:
     def allocate(self, n: int) -> list[int]:
         if n > len(self.free):
             raise InsufficientBlocksError(f"Insufficient free blocks: asked {n}, free {len(self.free)}")
-        return [self.free.popleft() for _ in range(n)]
+        blocks = [self.free.popleft() for _ in range(n)]
+        for b in blocks:
+            self._holders[b] = 1
+        return blocks
+
+    def fork(self, blocks: Sequence[int]) -> None:
+        """One more holder for each of `blocks`, all of which must be in use."""
+        missing = [b for b in blocks if b not in self._holders]
+        if missing:
+            raise ValueError(f"blocks {missing} are not in use")
+        for b in blocks:
+            self._holders[b] += 1
+
+    def holders(self, block: int) -> int:
+        """Holders of a block: 0 for a free one."""
+        return self._holders.get(block, 0)
 
     def release(self, blocks: list[int]) -> None:
-        self.free.extend(blocks)
+        for b in blocks:
+            n = self._holders.get(b, 1) - 1
+            if n > 0:
+                self._holders[b] = n
+            else:
+                self._holders.pop(b, None)
+                self.free.append(b)
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Renumber the used blocks into the lowest ids: returns (src, dst),
+        used blocks and the free ids below them that they take. The pages have
+        to be moved and every table rewritten before either is used again
+        (BlockCache.compact does both)."""
+        moves = []
+        for s, d in zip(sorted(self._holders, reverse=True), sorted(set(self.free))):
+            if d >= s:
+                break
+            moves.append((s, d))
+        if not moves:
+            return [], []
+        src, dst = (list(x) for x in zip(*moves))
+        self.free = deque(sorted(set(self.free).difference(dst).union(src)))
+        for s, d in moves:
+            self._holders[d] = self._holders.pop(s)
+        return src, dst
+
+
+def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple:
+    """The pools as la_copy_blocks takes them, from [L, NB, BS, Hkv, D] or one
+    layer's [NB, BS, Hkv, D]."""
+    _check(k_pool.dim() in (4, 5) and k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride()
+           and k_pool.dtype == v_pool.dtype and k_pool.device == v_pool.device,
+           "k_pool and v_pool must be [num_layers, num_blocks, block_size, num_heads_k, head_dim] (or one layer) of the "
+           "same shape, strides and type on one device")
+    _check(k_pool.stride(-1) == 1, "the head_dim axis must be contiguous")
+    layers, layer_stride = (k_pool.shape[0], k_pool.stride(0)) if k_pool.dim() == 5 else (1, 0)
+    nb, bs, heads, dim = k_pool.shape[-4:]
+    return (_ptr(k_pool), _ptr(v_pool), layer_stride, *k_pool.stride()[-4:-1], layers, nb, bs, heads, dim,
+            k_pool.element_size())
+
+
+def _check_ids(name: str, ids: torch.Tensor, n: int, device: torch.device) -> None:
+    _check(ids.dtype == torch.int32 and ids.shape == (n,) and ids.is_contiguous() and ids.device == device,
+           f"{name} must be a contiguous int32 [num_pairs] tensor on the pools' device")
+
+
+def _check_table(block_table: torch.Tensor, device: torch.device) -> None:
+    _check(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.device == device
+           and block_table.stride(1) == 1 and (block_table.shape[0] < 2 or block_table.stride(0) >= block_table.shape[1]),
+           "block_table must be row-contiguous int32 [batch, max_blocks] on the pools' device")
+
+
+def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
+                num_tokens: Optional[torch.Tensor] = None) -> None:
+    """Copy pages inside the pools: in every layer, K and V, the first
+    num_tokens[i] tokens of block src_blocks[i] (all of them without
+    num_tokens) to block dst_blocks[i], in one launch.
+
+    k_pool / v_pool: [L, NB, BS, Hkv, D] or one layer's [NB, BS, Hkv, D], of
+    any type of 1, 2 or 4 bytes. src_blocks, dst_blocks, num_tokens: int32 [n]
+    on the pools' device, read there. One block may be the source of several
+    copies. A copy whose destination is another's source, or the destination
+    of one before it, is skipped and recorded, as are ids outside the pool
+    (check_device_errors)."""
+    args = _pools(k_pool, v_pool)
+    device, n = k_pool.device, src_blocks.numel()
+    dev = _device_index(k_pool)
+    _check_ids("src_blocks", src_blocks, n, device)
+    _check_ids("dst_blocks", dst_blocks, n, device)
+    if num_tokens is not None:
+        _check_ids("num_tokens", num_tokens, n, device)
+    with torch.cuda.device(dev):
+        ensure_init(dev)
+        _lib.call("la_copy_blocks", *args, _ptr(src_blocks), _ptr(dst_blocks), _ptr(num_tokens), n,
+                  _ptr(error_word(dev)), _stream(device))
+
+
+def move_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
+                block_table: torch.Tensor) -> None:
+    """Move pages inside the pools: copy_blocks of whole pages, and every entry
+    src_blocks[i] of block_table (int32 [B, max_blocks] on the pools' device,
+    rewritten in place) becomes dst_blocks[i]. Entries of a move that is
+    skipped (see copy_blocks) stay as they are."""
+    args = _pools(k_pool, v_pool)
+    device, n = k_pool.device, src_blocks.numel()
+    dev = _device_index(k_pool)
+    _check_ids("src_blocks", src_blocks, n, device)
+    _check_ids("dst_blocks", dst_blocks, n, device)
+    _check_table(block_table, device)
+    rows, cols = block_table.shape
+    with torch.cuda.device(dev):
+        ensure_init(dev)
+        _lib.call("la_move_blocks", *args, _ptr(src_blocks), _ptr(dst_blocks), n,
+                  _ptr(block_table), block_table.stride(0) if rows > 1 else cols, rows, cols,
+                  _ptr(error_word(dev)), _stream(device))
+
+
+def shared_prefix_groups(tables: Sequence[Sequence[int]], lengths: Sequence[int], block_size: int,
+                         min_blocks: int = 1) -> tuple[list[int], list[int]]:
+    """The groups that flash_attn_with_shared_prefix takes, from the rows'
+    block tables: (prefix_lens, cu_prefix_rows). Consecutive rows whose tables
+    begin with the same block, filled by both, are one group; its prefix is
+    the run of blocks that all of them begin with and fill. Every row is in a
+    group: one that shares fewer than min_blocks blocks with its neighbours is
+    a group by itself, with a prefix of 0."""
+    lens, cu = [], [0]
+    rows = [list(t[: n // block_size]) for t, n in zip(tables, lengths)]
+    first = 0
+    while first < len(rows):
+        common, last = len(rows[first]), first + 1
+        while last < len(rows):
+            n = 0
+            while n < min(common, len(rows[last])) and rows[last][n] == rows[first][n]:
+                n += 1
+            if n < max(min_blocks, 1):
+                break
+            common, last = n, last + 1
+        lens.append(common * block_size if last - first > 1 else 0)
+        cu.append(last)
+        first = last
+    return lens, cu
 
 
 class BlockCache:
@@ -73,3 +221,55 @@ class BlockCache:
         if n > 1 and vt.stride(0) != n * vt.stride(1):
             vt = vt.contiguous()
         paged_kv_write(kt, vt, pos, block_tables, self.k[layer], self.v[layer])
+
+    def _upload(self, *lists: Sequence[int]) -> list[torch.Tensor]:
+        """int32 device tensors of equally long lists, in one copy."""
+        return list(torch.tensor(lists, dtype=torch.int32).to(self.device, non_blocking=True))
+
+    def copy_blocks(self, src: Sequence[int], dst: Sequence[int], num_tokens: Optional[Sequence[int]] = None) -> None:
+        """Copy blocks src[i] to dst[i] in every layer (the first num_tokens[i]
+        tokens of each, or all): copy_blocks for ids known on the host, which
+        are checked here."""
+        n, nb = len(src), self.k.shape[1]
+        if len(dst) != n or (num_tokens is not None and len(num_tokens) != n):
+            raise ValueError("src, dst and num_tokens differ in length")
+        if any(not 0 <= b < nb for b in (*src, *dst)):
+            raise ValueError(f"block ids outside the pool of {nb} blocks")
+        if len(set(dst)) != n or not set(dst).isdisjoint(src):
+            raise ValueError("every destination must be one copy's alone and no copy's source")
+        if num_tokens is not None and any(not 0 <= t <= self.block_size for t in num_tokens):
+            raise ValueError(f"num_tokens outside 0..{self.block_size}")
+        if n:
+            copy_blocks(self.k, self.v, *self._upload(*((src, dst) if num_tokens is None else (src, dst, num_tokens))))
+
+    def fork(self, allocator: BlockAllocator, blocks: Sequence[int], num_tokens: int, n: int = 1) -> list[list[int]]:
+        """The block tables of n children of a sequence that holds num_tokens
+        tokens in `blocks`: the whole blocks are shared (one more holder each),
+        a last block that is partly filled is copied to one of each child's
+        own, in one launch. Blocks behind num_tokens stay the parent's."""
+        full, rest = divmod(num_tokens, self.block_size)
+        if num_tokens < 0 or n < 0 or len(blocks) < full + (rest > 0):
+            raise ValueError(f"{len(blocks)} blocks do not hold {num_tokens} tokens")
+        if any(allocator.holders(b) == 0 for b in blocks[: full + (rest > 0)]):
+            raise ValueError("a block that is to be shared is not in use")
+        own = allocator.allocate(n) if rest else []
+        for i in range(n):
+            allocator.fork(blocks[:full])
+        if own:
+            self.copy_blocks([blocks[full]] * n, own, [rest] * n)
+        return [list(blocks[:full]) + own[i:i + 1] for i in range(n)]
+
+    def compact(self, allocator: BlockAllocator, block_table: Optional[torch.Tensor] = None) -> dict[int, int]:
+        """Move the used blocks to ids 1..n: the pages, the allocator's state
+        and the entries of a device block_table. Returns {old id: new id} of
+        the moved blocks, for tables on the host."""
+        if block_table is not None:
+            _check_table(block_table, self.k.device)
+        src, dst = allocator.compact()
+        if src:
+            s, d = self._upload(src, dst)
+            if block_table is None:
+                copy_blocks(self.k, self.v, s, d)
+            else:
+                move_blocks(self.k, self.v, s, d, block_table)
+        return dict(zip(src, dst))

@@ -15,7 +15,8 @@ Host rules shared by every entry point here:
   * nothing here synchronises the host, and the only allocations are the
     output tensors and a per-device workspace that is created on the first
     call and reused (so warm up once before CUDA-graph capture, exactly as
-    the engine does for flash-attn at leaninfer/engine/llm_engine.py:51-53).
+    the engine does for flash-attn at leaninfer/engine/llm_engine.py:51-53);
+    flash_attn_with_shared_prefix allocates its workspace with its output.
 """
 from __future__ import annotations
 
@@ -236,6 +237,87 @@ def flash_attn_with_kvcache(
             _ptr(lse),
             _ptr(ws), ws.numel(),
             _ptr(err), _stream(q.device),
+        )
+    return (out, lse) if return_softmax_lse else out
+
+
+def flash_attn_with_shared_prefix(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    block_table: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    cu_prefix_rows: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    return_softmax_lse: bool = False,
+):
+    """Paged GQA decode for a batch whose rows share long prefixes: the result
+    of flash_attn_with_kvcache on the same q, caches, cache_seqlens and
+    block_table, with the keys of a shared prefix read once for all the rows
+    that share it.
+
+    q: [B, 1, Hq, D] bf16; k_cache / v_cache: [num_blocks, block_size, Hkv, D]
+    bf16; cache_seqlens: int32 [B], the prefix included; block_table: int32
+    [B, max_blocks], the prefix's blocks first. Rows cu_prefix_rows[g] ..
+    cu_prefix_rows[g+1]-1 (int32 [G+1], ascending) are group g: their tables
+    hold the same blocks for their first prefix_lens[g] keys (int32 [G]), as
+    BlockCache.fork leaves them; shared_prefix_groups finds the groups of a
+    list of tables. Only whole blocks are taken as shared (prefix_lens is
+    rounded down). Rows in no group, empty groups and rows that end inside
+    the prefix are fine. All of it is read on the device: a captured graph
+    serves any division of the batch into at most G groups.
+    Returns out [B, 1, Hq, D] (and softmax_lse [B, Hq, 1] fp32 when asked).
+    Its workspace is allocated per call, so calls may overlap.
+    """
+    _check(q.dim() == 4 and q.shape[1] == 1, "q must be [batch, 1, num_heads, head_dim]")
+    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+           "k_cache and v_cache must be [num_blocks, block_size, num_heads_k, head_dim] of the same strides")
+    B, _, Hq, D = q.shape
+    Hkv = k_cache.shape[2]
+    _check(q.dtype == torch.bfloat16 and k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16,
+           "q, k_cache and v_cache must be bfloat16")
+    _check(q.stride(3) == 1 and k_cache.stride(3) == 1, "the head_dim axis must be contiguous")
+    _check(k_cache.shape[3] == D, "head_dim of q and k_cache differ")
+    _check(Hkv > 0 and Hq % Hkv == 0, "num_heads must be a multiple of num_heads_k")
+    _check(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B
+           and block_table.stride(1) == 1, "block_table must be row-contiguous int32 [batch, max_blocks]")
+    _check(cache_seqlens.dtype == torch.int32 and cache_seqlens.shape == (B,) and cache_seqlens.is_contiguous(),
+           "cache_seqlens must be a contiguous int32 [batch] tensor")
+    _check(cu_prefix_rows.dtype == torch.int32 and cu_prefix_rows.dim() == 1 and cu_prefix_rows.numel() >= 1
+           and cu_prefix_rows.is_contiguous(), "cu_prefix_rows must be a contiguous int32 [groups + 1] tensor")
+    G = cu_prefix_rows.numel() - 1
+    _check(prefix_lens.dtype == torch.int32 and prefix_lens.shape == (G,) and prefix_lens.is_contiguous(),
+           "prefix_lens must be a contiguous int32 [groups] tensor")
+    device = q.device
+    for t in (k_cache, v_cache, block_table, cache_seqlens, prefix_lens, cu_prefix_rows):
+        _check(t.device == device, "all tensors must be on one device")
+    dev = _device_index(q)
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    out = torch.empty((B, 1, Hq, D), dtype=q.dtype, device=device)
+    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=device) if return_softmax_lse else None
+    if B == 0:
+        return (out, lse) if return_softmax_lse else out
+    with torch.cuda.device(dev):
+        ensure_init(dev)
+        n = ctypes.c_size_t(0)
+        _lib.call("la_paged_decode_shared_prefix_workspace_size", dev, B, G, Hq, Hkv, D, ctypes.byref(n))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+        _lib.call(
+            "la_paged_decode_shared_prefix",
+            _ptr(q), q.stride(0), q.stride(2),
+            _ptr(k_cache), _ptr(v_cache),
+            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+            k_cache.shape[0], k_cache.shape[1],
+            _ptr(block_table), block_table.stride(0), block_table.shape[1],
+            _ptr(cache_seqlens),
+            _ptr(prefix_lens), _ptr(cu_prefix_rows), G,
+            B, Hq, Hkv, D,
+            ctypes.c_float(scale),
+            _ptr(out), out.stride(0), out.stride(2),
+            _ptr(lse),
+            _ptr(ws), n.value,
+            _ptr(error_word(dev)), _stream(device),
         )
     return (out, lse) if return_softmax_lse else out
 

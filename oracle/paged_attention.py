@@ -58,6 +58,33 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     return (out, lse) if return_lse else out
 
 
+def paged_decode_f64(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     cache_seqlens: torch.Tensor, softmax_scale: float | None = None):
+    """paged_decode in 64 bits, with what its error bounds are made of:
+    (out [B, 1, Hq, D], lse [B, Hq], absv, abss), absv the softmax-weighted
+    mean of |v| (as out), abss the largest scale * sum |q_d k_d| of a key (as
+    lse). A row without keys has zeros and lse -inf."""
+    B, _, Hq, D = q.shape
+    Hkv = k_cache.shape[2]
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale
+    out, absv = (torch.zeros(B, 1, Hq, D, dtype=torch.float64, device=q.device) for _ in range(2))
+    lse = torch.full((B, Hq), float("-inf"), dtype=torch.float64, device=q.device)
+    abss = torch.zeros(B, Hq, dtype=torch.float64, device=q.device)
+    for b in range(B):
+        ctx = int(cache_seqlens[b])
+        if ctx <= 0:
+            continue
+        k, v = (x.double() for x in gather_kv(k_cache, v_cache, block_table[b], ctx))
+        qb = q[b, 0].double().view(Hkv, Hq // Hkv, D) * scale
+        s = torch.einsum("hgd,thd->hgt", qb, k)
+        p = s.softmax(-1)
+        out[b, 0] = torch.einsum("hgt,thd->hgd", p, v).reshape(Hq, D)
+        absv[b, 0] = torch.einsum("hgt,thd->hgd", p, v.abs()).reshape(Hq, D)
+        lse[b] = s.logsumexp(-1).reshape(Hq)
+        abss[b] = torch.einsum("hgd,thd->hgt", qb.abs(), k.abs()).amax(-1).reshape(Hq)
+    return out, lse, absv, abss
+
+
 def paged_decode_padded(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                         cache_seqlens: torch.Tensor, softmax_scale: float | None = None):
     """The same decode math batched: gather every row's keys into a padded
