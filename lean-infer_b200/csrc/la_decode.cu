@@ -31,6 +31,7 @@
 #include <cstdint>
 #include <utility>
 
+#include "la_groups.cuh"
 #include "la_internal.h"
 #include "la_ptx.cuh"
 
@@ -103,6 +104,13 @@ struct Params {
   // (64, 16, Hkv, nsub, 1), whose rows land in the stage's order [sub-chunk
   // j][kv head][16 tokens]: a whole unit per half per tensor in one box.
   int unit_box;
+  // kPrefix: the rows' shared prefixes. Another pass covers those keys: row b
+  // reads the ones behind them, so its key positions and block-table columns
+  // are counted from there on (a prefix ends with a page). Rows that have a
+  // prefix, and rows split across CTAs, leave fp32 partials in slot
+  // (row + CTA), distinct for every part: from one part to the next along the
+  // line of units the row, the CTA or both go up by one.
+  PrefixGroups groups;
 };
 
 // Number of stage units of a sequence, with the same clamping everywhere.
@@ -115,6 +123,18 @@ __device__ __forceinline__ int seq_ctx(const Params& p, int b) {
     c = static_cast<int>(cap);
   }
   return c;
+}
+// Keys that row b reads by itself, and (kPrefix) the blocks before them.
+template <bool kPrefix>
+__device__ __forceinline__ int own_keys(const Params& p, int b, int* block0 = nullptr) {
+  const int ctx = seq_ctx(p, b);
+  if constexpr (!kPrefix) {
+    return ctx;
+  } else {
+    const int n = prefix_keys(p.groups, b, ctx);
+    if (block0) *block0 = p.bs_shift >= 0 ? (n >> p.bs_shift) : (n / p.block_size);
+    return ctx - n;
+  }
 }
 __device__ __forceinline__ int units_of(int ctx, int tc) { return (ctx + tc - 1) / tc; }
 // Division by the block size and the unit size on the producer's per-unit
@@ -140,11 +160,12 @@ __device__ __forceinline__ float warp_sum_g(float v) {
 }
 
 // Total units over all sequences, computed by one warp.
+template <bool kPrefix>
 __device__ long long total_units(const Params& p, int lane) {
   long long tot = 0;
   for (int base = 0; base < p.batch; base += 32) {
     const int b = base + lane;
-    int n = (b < p.batch) ? units_of(seq_ctx(p, b), p.tc) : 0;
+    int n = (b < p.batch) ? units_of(own_keys<kPrefix>(p, b), p.tc) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     tot += n;
@@ -160,7 +181,14 @@ __device__ long long total_units(const Params& p, int lane) {
 // registers (a scan per 32 sequences, one after another, took 18k clocks at
 // 1024 sequences before the first copy could be issued).
 __device__ __forceinline__ long long cta_start(long long c, long long T, long long G);
-template <int kChunks>
+// CTAs that the units are divided among. kPrefix: no more than there are
+// units, so that every one of them has some and a row's parts are those of
+// consecutive CTAs.
+template <bool kPrefix>
+__device__ __forceinline__ long long parts_of(long long T, long long grid) {
+  return kPrefix && T < grid ? (T > 0 ? T : 1) : grid;
+}
+template <int kChunks, bool kPrefix>
 __device__ __forceinline__ void split_from_regs(const Params& p, int lane, const int (&un)[kChunks], long long& T,
                                                 long long& u0, long long& u1, int& b0, long long& pb0) {
   long long own = 0;
@@ -174,9 +202,10 @@ __device__ __forceinline__ void split_from_regs(const Params& p, int lane, const
   }
   const long long excl = incl - own;
   T = __shfl_sync(0xffffffffu, incl, 31);
-  const long long G = gridDim.x;
+  const long long G = parts_of<kPrefix>(T, gridDim.x);
   u0 = cta_start(blockIdx.x, T, G);
   u1 = cta_start(blockIdx.x + 1, T, G);
+  if (kPrefix && blockIdx.x >= G) u0 = u1 = T;
   b0 = p.batch;
   pb0 = T;
   if (u1 <= u0) return;
@@ -233,7 +262,12 @@ __device__ __forceinline__ long long cta_of(long long x, long long T, long long 
 // kChunks: the split is held in registers for up to 32 x kChunks sequences
 // (8 for the engine's batches, 32 for the many short rows of the KV-head-
 // sharded partition).
-template <int kStages, int kChunks>
+// kPrefix: every row's keys behind its shared prefix. That grid is launched
+// behind the one that covers the prefixes, which lets it start as soon as the
+// kernels before them both are done: it reads nothing of the prefix pass, so
+// it waits for that grid only at its end, for the sake of the pass that reads
+// both grids' partials.
+template <int kStages, int kChunks, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k1,
@@ -283,12 +317,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const long long c = raw[i] < 0 ? 0 : (raw[i] > cap ? cap : raw[i]);
-      un[i] = units_of(static_cast<int>(c), p.tc);
+      if constexpr (kPrefix) {
+        // rows past the batch have no keys
+        const int own = static_cast<int>(c) - (c > 0 ? prefix_keys(p.groups, lane * kChunks + i, static_cast<int>(c)) : 0);
+        un[i] = units_of(own, p.tc);
+      } else {
+        un[i] = units_of(static_cast<int>(c), p.tc);
+      }
     }
-    split_from_regs(p, lane, un, sT, su0, su1, sb0, spb0);
+    split_from_regs<kChunks, kPrefix>(p, lane, un, sT, su0, su1, sb0, spb0);
   }
   // Everything below may read data written by the previous kernel in the stream.
-  grid_dependency_wait();
+  if constexpr (!kPrefix) grid_dependency_wait();
 
   // Producer lookups go through two windows held across its 32 lanes, so
   // that a unit's copies wait on no global load in the common case: lane i
@@ -300,15 +340,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   // windows of the first sequence are loaded with the speculative split,
   // together with the re-read that checks it.
   int sb = 0, swin = 0, bb = -1, wl = 0, bwin = -1;
+  int owin = 0;  // kPrefix: the blocks before the sequence's own keys, beside swin
   auto load_swin = [&](int base) {
     sb = base;
-    swin = (sb + lane < p.batch) ? seq_ctx(p, sb + lane) : 0;
+    swin = (sb + lane < p.batch) ? own_keys<kPrefix>(p, sb + lane, &owin) : 0;
+  };
+  // The first block of sequence `seq` that it reads by itself.
+  auto block0_of = [&](int seq) -> int {
+    if constexpr (!kPrefix) return 0;
+    if (seq >= sb && seq < sb + 32) return __shfl_sync(0xffffffffu, owin, seq - sb);  // warp-uniform branch
+    int o = 0;
+    if (seq < p.batch) own_keys<kPrefix>(p, seq, &o);
+    return o;
   };
   auto load_bwin = [&](int seq, int first) {
     bb = seq;
     wl = first;
-    bwin = (seq < p.batch && wl + lane < p.max_blocks)
-               ? p.block_table[static_cast<long long>(seq) * p.bt_stride + wl + lane]
+    const int o = block0_of(seq);
+    bwin = (seq < p.batch && o + wl + lane < p.max_blocks)
+               ? p.block_table[static_cast<long long>(seq) * p.bt_stride + o + wl + lane]
                : -1;
   };
   if (warp >= kCWarps) {
@@ -317,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       load_bwin(sb0, static_cast<int>((su0 - spb0) * p.tc / p.block_size));
     }
     bool same = spec;
-    if (spec) {
+    if (spec && !kPrefix) {
       int now[kChunks];
       load_lens(p, lane, now);
 #pragma unroll
@@ -326,17 +376,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       same = __all_sync(0xffffffffu, same);
     }
     // Partition: this CTA's unit range and the sequence it starts in.
-    const long long T = same ? sT : total_units(p, lane);
-    const long long G = gridDim.x;
-    const long long u0 = same ? su0 : cta_start(blockIdx.x, T, G);
-    const long long u1 = same ? su1 : cta_start(blockIdx.x + 1, T, G);
+    const long long T = same ? sT : total_units<kPrefix>(p, lane);
+    const long long G = parts_of<kPrefix>(T, gridDim.x);
+    const bool idle = kPrefix && blockIdx.x >= G;
+    const long long u0 = same ? su0 : idle ? T : cta_start(blockIdx.x, T, G);
+    const long long u1 = same ? su1 : idle ? T : cta_start(blockIdx.x + 1, T, G);
     long long acc = 0;
     int b0 = same ? sb0 : p.batch;
     long long pb0 = same ? spb0 : T;
     if (!same && u1 > u0) {
       for (int base = 0; base < p.batch; base += 32) {
         const int b = base + lane;
-        const int n = (b < p.batch) ? units_of(seq_ctx(p, b), p.tc) : 0;
+        const int n = (b < p.batch) ? units_of(own_keys<kPrefix>(p, b), p.tc) : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -422,8 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (nbb <= b) {  // read at the next sequence change, not before
           nbb = b + 1;
-          nbwin = (nbb < p.batch && lane < p.max_blocks)
-                      ? p.block_table[static_cast<long long>(nbb) * p.bt_stride + lane]
+          const int o = block0_of(nbb);
+          nbwin = (nbb < p.batch && o + lane < p.max_blocks)
+                      ? p.block_table[static_cast<long long>(nbb) * p.bt_stride + o + lane]
                       : -1;
         }
       }
@@ -456,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const unsigned act = __ballot_sync(0xffffffffu, active);
+      const int shared = block0_of(b);
       if (lane == 0) {
         StageDesc d;
         d.b = b;
@@ -464,9 +517,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         int flags = 0;
         if (k == 0 || uis == 0) flags |= kFlagFirst;
         if (k == nu - 1 || uis == nb - 1) flags |= kFlagLast;
-        if (seq_k0 >= 0 && seq_k0 + nb <= nu) flags |= kFlagWhole;
+        if (seq_k0 >= 0 && seq_k0 + nb <= nu && shared == 0) flags |= kFlagWhole;
         d.flags = flags;
-        d.slot = 2 * static_cast<int>(blockIdx.x) + (seq_k0 <= 0 ? 0 : 1);
+        d.slot = kPrefix ? b + static_cast<int>(blockIdx.x)
+                         : 2 * static_cast<int>(blockIdx.x) + (seq_k0 <= 0 ? 0 : 1);
         descs[s] = d;
         // Q is read only on a sequence's first unit (kFlagFirst): load it there.
         const bool first = (flags & kFlagFirst) != 0;
@@ -537,6 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int kk = (k > kStages ? k - kStages : 0); kk < k; ++kk)
         if (kk % nprod == pid) mbar_wait(&full[kk % kStages], static_cast<uint32_t>((kk / kStages) & 1), nullptr, 0);
     }
+    if constexpr (kPrefix) grid_dependency_wait();
     return;
   }
 
@@ -670,6 +725,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (d.flags & kFlagLast) {
       float L0 = warp_sum_g(l0), L1 = warp_sum_g(l1);
+      // kPrefix: a sum that is NaN counts, so that it reaches the result
+      auto some = [](float l) { return kPrefix ? l != 0.f : l > 0.f; };
       const int c0 = 2 * tq, c1 = 2 * tq + 1;
       bool writer = true;
       if (p.nsub > 1) {
@@ -762,8 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (p.lse_out && g == 0) {
           const float ln2 = 0.6931471805599453f;
-          if (c0 < G) p.lse_out[static_cast<long long>(d.b) * p.hq + h * G + c0] = L0 > 0.f ? (m0 + __log2f(L0)) * ln2 : NEG_INF;
-          if (c1 < G) p.lse_out[static_cast<long long>(d.b) * p.hq + h * G + c1] = L1 > 0.f ? (m1 + __log2f(L1)) * ln2 : NEG_INF;
+          if (c0 < G) p.lse_out[static_cast<long long>(d.b) * p.hq + h * G + c0] = some(L0) ? (m0 + __log2f(L0)) * ln2 : NEG_INF;
+          if (c1 < G) p.lse_out[static_cast<long long>(d.b) * p.hq + h * G + c1] = some(L1) ? (m1 + __log2f(L1)) * ln2 : NEG_INF;
         }
       } else if (writer) {
         float* po = p.part_o + static_cast<long long>(d.slot) * p.hq * kD;
@@ -785,8 +842,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (g == 0) {
           float* pl = p.part_lse + static_cast<long long>(d.slot) * p.hq;
-          if (c0 < G) pl[h * G + c0] = L0 > 0.f ? m0 + __log2f(L0) : NEG_INF;
-          if (c1 < G) pl[h * G + c1] = L1 > 0.f ? m1 + __log2f(L1) : NEG_INF;
+          if (c0 < G) pl[h * G + c0] = some(L0) ? m0 + __log2f(L0) : NEG_INF;
+          if (c1 < G) pl[h * G + c1] = some(L1) ? m1 + __log2f(L1) : NEG_INF;
         }
       }
     }
@@ -1095,16 +1152,22 @@ static int grid_for(int device) { return num_sms(device); }
 
 }  // namespace decode
 
+template <int kStages, int kChunks>
+static cudaError_t init_instances(int smem) {
+  const cudaError_t e = cudaFuncSetAttribute(decode::paged_decode_kernel<kStages, kChunks, false>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(decode::paged_decode_kernel<kStages, kChunks, true>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+}
+
 int decode_init(int device) {
   (void)device;
   const int lim = 227 * 1024;
-  cudaError_t e = cudaFuncSetAttribute(decode::paged_decode_kernel<3, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(decode::paged_decode_kernel<2, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(decode::paged_decode_kernel<3, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(decode::paged_decode_kernel<2, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
+  cudaError_t e = init_instances<3, 8>(lim);
+  if (e == cudaSuccess) e = init_instances<2, 8>(lim);
+  if (e == cudaSuccess) e = init_instances<3, 32>(lim);
+  if (e == cudaSuccess) e = init_instances<2, 32>(lim);
   if (e == cudaSuccess) {
     cudaFuncAttributes a;
     e = cudaFuncGetAttributes(&a, decode::paged_decode_combine_kernel<false>);
@@ -1145,7 +1208,8 @@ static int paged_decode_impl(const void* q, int64_t q_batch_stride, int64_t q_he
                              const int32_t* cache_seqlens, int batch, int num_q_heads, int num_kv_heads,
                              int head_dim, float softmax_scale, void* out, int64_t out_batch_stride,
                              int64_t out_head_stride, float* softmax_lse, void* workspace, size_t workspace_bytes,
-                             int* dev_error, cudaStream_t stream, const PeerOut* peers) {
+                             int* dev_error, cudaStream_t stream, const PeerOut* peers,
+                             const OwnKeysPass* own = nullptr) {
   if (!q || !k_cache || !v_cache || !block_table || !cache_seqlens || !out) return LA_ERR_INVALID_ARGUMENT;
   if (batch < 0 || num_blocks <= 0 || block_size <= 0 || max_blocks_per_seq <= 0) return LA_ERR_INVALID_ARGUMENT;
   if (batch == 0) return LA_OK;
@@ -1174,7 +1238,7 @@ static int paged_decode_impl(const void* q, int64_t q_batch_stride, int64_t q_he
   size_t need = 0;
   int st = la_paged_decode_workspace_size(device, num_q_heads, num_kv_heads, head_dim, &need);
   if (st != LA_OK) return st;
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return LA_ERR_WORKSPACE;
+  if (!own && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return LA_ERR_WORKSPACE;
 
   CUtensorMap tq, tk, tv, tk1, tv1;
   {
@@ -1271,6 +1335,12 @@ static int paged_decode_impl(const void* q, int64_t q_batch_stride, int64_t q_he
   const size_t o_bytes = (slots * num_q_heads * kD * sizeof(float) + 255) & ~size_t(255);
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + o_bytes);
+  p.groups = PrefixGroups{};
+  if (own) {
+    p.groups = own->groups;
+    p.part_o = own->part_o;
+    p.part_lse = own->part_lse;
+  }
   p.err = dev_error;
   // Each Q half tile starts on a 1024-byte boundary (the 128-byte swizzle atom).
   p.big_box = big_box == 1;
@@ -1286,13 +1356,14 @@ static int paged_decode_impl(const void* q, int64_t q_batch_stride, int64_t q_he
   // one-kv-head rows it took the pipeline off the producer's path); with a
   // few short sequences (B = 8) the extra warp measured slower.
   const int threads = (kCWarps + (batch >= 16 ? 2 : 1)) * 32;
-  cudaError_t e;
-  if (stages == 3)
-    e = batch <= 256 ? launch_pdl(paged_decode_kernel<3, 8>, dim3(grid), dim3(threads), smem, stream, tq, tk, tv, tk1, tv1, p)
-                     : launch_pdl(paged_decode_kernel<3, 32>, dim3(grid), dim3(threads), smem, stream, tq, tk, tv, tk1, tv1, p);
-  else
-    e = batch <= 256 ? launch_pdl(paged_decode_kernel<2, 8>, dim3(grid), dim3(threads), smem, stream, tq, tk, tv, tk1, tv1, p)
-                     : launch_pdl(paged_decode_kernel<2, 32>, dim3(grid), dim3(threads), smem, stream, tq, tk, tv, tk1, tv1, p);
+  auto launch = [&](auto* k3, auto* k2) {
+    return launch_pdl(stages == 3 ? k3 : k2, dim3(grid), dim3(threads), smem, stream, tq, tk, tv, tk1, tv1, p);
+  };
+  if (own)
+    return cuda_status(batch <= 256 ? launch(paged_decode_kernel<3, 8, true>, paged_decode_kernel<2, 8, true>)
+                                    : launch(paged_decode_kernel<3, 32, true>, paged_decode_kernel<2, 32, true>));
+  cudaError_t e = batch <= 256 ? launch(paged_decode_kernel<3, 8, false>, paged_decode_kernel<2, 8, false>)
+                               : launch(paged_decode_kernel<3, 32, false>, paged_decode_kernel<2, 32, false>);
   if (e != cudaSuccess) return cuda_status(e);
   // peer stores: kCombinePeerWarps heads per CTA (fewer when they do not divide the heads)
   int wpc = 1;
@@ -1312,6 +1383,21 @@ static int paged_decode_impl(const void* q, int64_t q_batch_stride, int64_t q_he
 }
 
 }  // namespace decode
+
+int decode_own_keys(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_cache,
+                    const void* v_cache, int64_t kv_block_stride, int64_t kv_token_stride, int64_t kv_head_stride,
+                    int64_t num_blocks, int block_size, const int32_t* block_table, int64_t bt_seq_stride,
+                    int max_blocks_per_seq, const int32_t* cache_seqlens, int batch, int num_q_heads,
+                    int num_kv_heads, int head_dim, float softmax_scale, void* out, int64_t out_batch_stride,
+                    int64_t out_head_stride, float* softmax_lse, int* dev_error, cudaStream_t stream,
+                    const OwnKeysPass& own) {
+  return decode::paged_decode_impl(q, q_batch_stride, q_head_stride, k_cache, v_cache, kv_block_stride,
+                                   kv_token_stride, kv_head_stride, num_blocks, block_size, block_table,
+                                   bt_seq_stride, max_blocks_per_seq, cache_seqlens, batch, num_q_heads, num_kv_heads,
+                                   head_dim, softmax_scale, out, out_batch_stride, out_head_stride, softmax_lse,
+                                   nullptr, 0, dev_error, stream, nullptr, &own);
+}
+
 }  // namespace la
 
 extern "C" int la_paged_decode(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_cache,

@@ -50,5 +50,6 @@ int decode_init(int device);
 int pre_attn_init(int device);
 int prefill_init(int device);
 int oproj_init(int device);
+int prefix_init(int device);
 
 }  // namespace la
