@@ -5,35 +5,43 @@
 // cu_prefix_rows[g] .. cu_prefix_rows[g+1]-1 hold the same pages for their
 // first keys, so the softmax is taken in two parts, joined by their maxima and
 // sums: over the shared keys for all rows of a group at once, as matrix
-// products (prefix_kernel), and over each row's own keys (the decode kernel of
-// la_decode.cu). combine_kernel joins the parts of every row.
+// products, and over each row's own keys behind them, streamed row by row
+// (the warps of la_decode_body.cuh).
 //
-// prefix_kernel. For one kv head the group's rows x query heads of the kv head
+// shared_prefix_kernel does both at once, each on its own SMs. The shared part
+// is bound by the tensor cores and the exponentials when many rows share a
+// prefix (a step, see below, takes ~2.4 us on an SM); the rows' own keys are
+// bound by HBM, which about 64 SMs of streaming CTAs already draw 4.75 of its
+// ~6 TB/s from (96: 5.7). One after the other on all SMs, the two took their
+// sum, and each its own start (128 rows behind 32768 keys: 103 us); side by
+// side they take little more than the longer one. Every CTA counts the steps
+// and units of both parts and takes the same decision: P CTAs for the prefixes,
+// as many as finish with the rest by this model, the others for the rows.
+// combine_kernel joins the parts of every row.
+//
+// Shared part. For one kv head the group's rows x query heads of the kv head
 // are the rows of Q; with 128-key tiles of K and V,
 //   S = Q K^T,  P = exp2(S * scale * log2 e - m),  O += P V,  l += sum P
 // run on tcgen05 with fp32 accumulators in tensor memory, m the running row
-// maximum. Bound by HBM (the prefix once) while a kv head has at most ~256
-// query rows, by the tensor cores and the exponentials above that.
-//
-// Work. An item is (group, kv head, pair of 128-row tiles); both tiles use
+// maximum. An item is (group, kv head, pair of 128-row tiles); both tiles use
 // each K/V tile that is staged. Where only one tile is left over, its two
 // accumulators take the even and the odd key tiles instead, so that one
 // tile's products still run while the other's exponentials do. A step is two
 // tile products either way: one key tile of a pair of row tiles, or two key
 // tiles of a single one. The steps of all items, laid end to end, are cut into
-// equal ranges, one per CTA (one CTA per SM), whatever the number of groups;
-// an item's part in a range is a segment, which leaves normalised fp32 O rows
-// and base-2 logarithms of its sums. Everything is found on the device, so the
-// launch does not depend on the groups.
+// P equal ranges; an item's part in a range is a segment, which leaves
+// normalised fp32 O rows and base-2 logarithms of its sums.
 //
-// CTA, 16 warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread per row, the S
-// row in registers), 8-11 store the segments' O, 12 issues the products, 13
-// the TMA loads. Tensor memory: S0 S1 O0 O1, 128 columns each; P over S.
+// CTA, 16 warps. Shared part: 0-3 and 4-7 softmax of tile 0 and 1 (a thread
+// per row, the S row in registers), 8-11 store the segments' O, 12 issues the
+// products, 13 the TMA loads; tensor memory holds S0 S1 O0 O1, 128 columns
+// each, P over S. Own keys: 0-7 consume, 8 and 9 load.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
+#include "la_decode_body.cuh"
 #include "la_groups.cuh"
 #include "la_internal.h"
 #include "la_ptx.cuh"
@@ -52,35 +60,52 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;        // O_t at kColO + 128 t; S_t at 128 t
 constexpr uint32_t kIdescQK = idesc_bf16_f32(128, kKeys, false, false);
 constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, false, true);
-constexpr int kRegSoftmax = 160, kRegStore = 88, kRegOther = 104;
-static_assert(256 * kRegSoftmax + 128 * kRegStore + 128 * kRegOther <= kThreads * 128,
+// Registers per thread, of the 512 x 128 that the CTA is launched with.
+constexpr int kRegSoftmax = 160, kRegStore = 88, kRegOther = 104;  // shared part: warps 0-7, 8-11, 12-15
+constexpr int kRegConsume = 160, kRegLoad = 104, kRegIdle = 88;    // own keys: the same
+static_assert(256 * kRegSoftmax + 128 * kRegStore + 128 * kRegOther <= kThreads * 128 &&
+                  256 * kRegConsume + 128 * kRegLoad + 128 * kRegIdle <= kThreads * 128,
               "the register split must fit in the registers the CTA is launched with");
-// Shared memory: Q0 Q1 | K/V ring | staging of O (4 KB per storing warp) |
-// row sums and maxima | barriers and the CTA's range.
-constexpr int kOffKV = 2 * kTile;
+// Shared memory. Control, both parts' barriers apart: they are initialised
+// before the CTA knows which part it takes. Then the part's data: Q0 Q1, K/V
+// ring, staging of O (4 KB per storing warp), row sums and maxima; or the
+// stages and the merge area of the decode warps.
+constexpr int kOffOwnBar = 256;
+constexpr int kOffPlan = 384;
+constexpr int kOffDesc = 512;
+constexpr int kOffZero = 640;
+constexpr int kOffWalk = 768;          // of the softmax warps, kept out of their registers
+constexpr int kWalkBytes = 112;
+constexpr int kOffTable = 2048;
+constexpr int kMaxGroups = 512;        // groups that the table holds; more are read from global memory
+constexpr int kCtrlBytes = 8192;
+constexpr int kOffQ = kCtrlBytes;
+constexpr int kOffKV = kOffQ + 2 * kTile;
 constexpr int kOffStage = kOffKV + kStages * kTile;
 constexpr int kStageBytes = 32 * 128;
 constexpr int kOffStats = kOffStage + 4 * kStageBytes;
-constexpr int kOffBar = kOffStats + 2 * 2 * kRows * 4;
-constexpr int kOffWalk = kOffBar + 256;  // of the softmax warps, kept out of their registers
-constexpr int kWalkBytes = 112;
-constexpr size_t kSmemBytes = kOffWalk + 8 * kWalkBytes + 1024;  // + alignment to 1024 bytes at run time
+constexpr size_t kSmemBytes = kOffStats + 2 * 2 * kRows * 4 + 1024;  // + alignment to 1024 bytes at run time
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+static_assert(kOffWalk + 8 * kWalkBytes <= kOffTable && kOffTable + kMaxGroups * sizeof(PrefixGroup) <= kCtrlBytes,
+              "control area");
+
+// The time model that divides the SMs (microseconds; measured on a B200 at
+// ~1.9 GHz): a step of the shared part; a unit of 64 KB of a row's own keys
+// on one SM, without and with sub-chunks to merge (nsub > 1); 64 KB at the
+// rate that all SMs together reach.
+constexpr float kStepUs = 2.4f, kUnitUs = 0.8f, kUnitMergedUs = 1.25f, kHbmUs = 0.0109f;
 
 struct Params {
-  PrefixGroups groups;
-  const int* table;
-  long long table_stride;
-  int max_blocks;
-  int num_blocks;
-  int box_keys;  // keys per TMA box, a power of two that divides the block size
-  int hkv, group;
-  int per_tile;   // sequences per row tile: 128 / group
-  float scale_log2;
-  float* part_o;    // [rows][D]
-  float* part_lse;  // [rows], base 2
-  int* err;
+  decode::Params own;  // the rows' own keys; groups, tables, counts and scale of both parts
+  int box_keys;        // keys per TMA box, a power of two that divides the block size
+  int per_tile;        // sequences per row tile: 128 / group
+  float* part_o;       // [rows][D]
+  float* part_lse;     // [rows], base 2
+  int4* items;         // [batch][hkv]: first partial row of the row's first head, distance of the second
+                       // accumulator's (0: none), first and last CTA of its item
+  int* flags;          // [batch]: kShares, kOwn
 };
+constexpr int kShares = 1, kOwn = 2;
 
 // How the steps of a group lie: kv heads one after another, in each the pairs
 // of row tiles, the single tile last.
@@ -101,16 +126,8 @@ __device__ __forceinline__ Shape shape_of(const PrefixGroup& g, int per_tile) {
   return s;
 }
 
-__device__ __forceinline__ int steps_of(const Params& p, int g) {
-  const PrefixGroup r = prefix_group(p.groups, g);
-  return r.keys > 0 ? p.hkv * shape_of(r, p.per_tile).per_head : 0;
-}
-
-// The even split of T steps or units over at most `grid` CTAs, each with some.
-__device__ __forceinline__ long long parts_of(long long T, int grid) { return T < grid ? (T > 0 ? T : 1) : grid; }
-__device__ __forceinline__ long long part_start(long long c, long long T, long long G) { return c * T / G; }
-__device__ __forceinline__ int part_of(long long x, long long T, long long G) {
-  return static_cast<int>(((x + 1) * G - 1) / T);
+__device__ __forceinline__ int steps_of(const Params& p, const PrefixGroup& g) {
+  return g.keys > 0 ? p.own.hkv * shape_of(g, p.per_tile).per_head : 0;
 }
 
 // First partial row of item (g, h, r) in CTA c. An item's segments take up to
@@ -118,15 +135,171 @@ __device__ __forceinline__ int part_of(long long x, long long T, long long G) {
 // line of steps the item, the CTA or both go up, the item by at least the rows
 // that one segment of it takes.
 __device__ __forceinline__ int part_row(const Params& p, const PrefixGroup& g, int h, int r, int c) {
-  return 2 * p.group * (p.hkv * g.first + h * g.rows + r * 2 * p.per_tile) + 2 * kRows * c;
+  return 2 * p.own.group * (p.own.hkv * g.first + h * g.rows + r * 2 * p.per_tile) + 2 * kRows * c;
 }
 
-// The CTA's range of steps and where it begins.
-struct Range {
-  long long u0, u1;  // steps
-  long long before;  // steps before group g0
-  int g0;
+// What the CTA does: its range of steps (P > blockIdx.x) or of units, and
+// where that begins.
+struct Plan {
+  long long u0, u1;
+  long long before;  // steps before group `at`, or units before row `at`
+  int at;
+  int P;             // CTAs of the shared part
 };
+
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+// Lengths of rows base + 8 lane + i (0 past the batch), 16 bytes at a time
+// where they can be.
+__device__ __forceinline__ void load_lens8(const Params& p, int lane, int base, int (&raw)[8]) {
+  const int* s = p.own.seqlens;
+  const int b0 = base + 8 * lane;
+  const bool vec = (reinterpret_cast<uintptr_t>(s) & 15) == 0;
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const int b = b0 + 4 * v;
+    if (vec && b + 3 < p.own.batch) {
+      const int4 x = *reinterpret_cast<const int4*>(s + b);
+      raw[4 * v] = x.x;
+      raw[4 * v + 1] = x.y;
+      raw[4 * v + 2] = x.z;
+      raw[4 * v + 3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[4 * v + e] = b + e < p.own.batch ? s[b + e] : 0;
+    }
+  }
+}
+
+// Units of those rows (kept in raw), and their sum.
+__device__ __forceinline__ int units8(const Params& p, const PrefixGroup* tab, int lane, int base, int (&raw)[8]) {
+  int sum = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    int c = raw[0];
+    c = c < 0 ? 0 : c > p.own.groups.cap ? static_cast<int>(p.own.groups.cap) : c;
+    if (c > 0) c -= prefix_keys(p.own.groups, tab, base + 8 * lane + i, c);
+    const int n = decode::units_p(p.own, c);
+    sum += n;
+#pragma unroll
+    for (int e = 0; e < 7; ++e) raw[e] = raw[e + 1];  // the loop is kept short: its code is cold
+    raw[7] = n;
+  }
+  return sum;
+}
+
+// One warp's work. tab: the table to fill, or null where the groups exceed it.
+__device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, int lane) {
+  const PrefixGroups& G = p.own.groups;
+  int raw[8];
+  load_lens8(p, lane, 0, raw);
+  // the shared part: steps, and key tiles that are read
+  long long S = 0, tiles = 0;
+  for (int b = 0; b < G.n; b += 32) {
+    const int g = b + lane;
+    int s = 0, t = 0;
+    if (g < G.n) {
+      const PrefixGroup r = load_group(G, g);
+      if (tab) tab[g] = r;
+      if (blockIdx.x == 0 && p.own.err && (r.first < 0 || G.cu[g + 1] < r.first || G.cu[g + 1] > G.batch))
+        atomicCAS(p.own.err, 0, LA_DEVERR_PREFIX);
+      s = steps_of(p, r);
+      t = p.own.hkv * ((r.keys + kKeys - 1) / kKeys);
+    }
+    S += warp_sum(s);
+    tiles += warp_sum(t);
+  }
+  __syncwarp();
+  // the rows' own keys: units
+  long long U = 0;
+  const int first = units8(p, tab, lane, 0, raw);
+  U = warp_sum(first);
+  for (int base = 256; base < G.batch; base += 256) {
+    int x[8];
+    load_lens8(p, lane, base, x);
+    U += warp_sum(units8(p, tab, lane, base, x));
+  }
+  const int grid = static_cast<int>(gridDim.x);
+  const float a = static_cast<float>(S) * kStepUs;
+  const float own = static_cast<float>(U) * (p.own.nsub > 1 ? kUnitMergedUs : kUnitUs);
+  const float T = fmaxf(static_cast<float>(U + tiles) * kHbmUs, (a + own) / static_cast<float>(grid));
+  Plan r;
+  r.P = 0;
+  if (S > 0) {
+    const int most = grid - (U > 0 ? 1 : 0);
+    r.P = max(1, min(static_cast<int>(ceilf(a / T)), static_cast<int>(S < most ? S : most)));
+  }
+  r.u0 = r.u1 = r.before = 0;
+  r.at = 0;
+  const int c = static_cast<int>(blockIdx.x);
+  if (c < r.P) {
+    r.u0 = decode::cta_start(c, S, r.P);
+    r.u1 = decode::cta_start(c + 1, S, r.P);
+    long long acc = 0;
+    for (int b = 0; b < G.n; b += 32) {  // the group of the first step
+      const int s = b + lane < G.n ? steps_of(p, prefix_group(G, tab, b + lane)) : 0;
+      const int incl = warp_scan(s, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        r.at = b + src;
+        r.before = acc + __shfl_sync(0xffffffffu, incl - s, src);
+        break;
+      }
+      acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  } else {
+    // no more CTAs than units, so that a row's parts are those of consecutive ones
+    const long long Q = U < grid - r.P ? U : grid - r.P;
+    if (c - r.P < Q) {
+      r.u0 = decode::cta_start(c - r.P, U, Q);
+      r.u1 = decode::cta_start(c - r.P + 1, U, Q);
+      long long acc = 0;
+      for (int base = 0; base < G.batch; base += 256) {  // the row of the first unit
+        int sum = first;
+        if (base > 0) {
+          load_lens8(p, lane, base, raw);
+          sum = units8(p, tab, lane, base, raw);
+        }
+        const int incl = warp_scan(sum, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          int at = 0;
+          long long before = acc + incl - sum;
+          if (lane == src) {
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              found |= r.u0 < before + raw[i];
+              if (!found) {
+                before += raw[i];
+                at = i + 1;
+              }
+            }
+          }
+          r.at = base + 8 * src + __shfl_sync(0xffffffffu, at, src);
+          r.before = __shfl_sync(0xffffffffu, before, src);
+          break;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+  }
+  return r;
+}
 
 // Segments of the CTA's range, one after another (the same in every thread).
 struct Walk {
@@ -144,18 +317,19 @@ struct Segment {
   int tile0, tiles; // key tiles
   int keys;         // of the group
   int row0;         // first partial row
+  int begin, end;   // of the item
 };
 
-__device__ __forceinline__ void walk_group(const Params& p, Walk& w, int g) {
+__device__ __forceinline__ void walk_group(const Params& p, const PrefixGroup* tab, Walk& w, int g) {
   w.g = g;
-  w.grp = prefix_group(p.groups, g);
+  w.grp = prefix_group(p.own.groups, tab, g);
   w.shp = shape_of(w.grp, p.per_tile);
 }
 
-__device__ __forceinline__ void walk_start(const Params& p, const Range& R, Walk& w) {
+__device__ __forceinline__ void walk_start(const Params& p, const PrefixGroup* tab, const Plan& R, Walk& w) {
   w.left = static_cast<int>(R.u1 - R.u0);
   if (w.left <= 0) return;
-  walk_group(p, w, R.g0);
+  walk_group(p, tab, w, R.at);
   const int x = static_cast<int>(R.u0 - R.before);
   w.h = x / w.shp.per_head;
   const int y = x - w.h * w.shp.per_head;
@@ -163,7 +337,7 @@ __device__ __forceinline__ void walk_start(const Params& p, const Range& R, Walk
   w.s = y - w.r * w.shp.tiles;
 }
 
-__device__ __forceinline__ bool walk_next(const Params& p, Walk& w, Segment& e) {
+__device__ __forceinline__ bool walk_next(const Params& p, const PrefixGroup* tab, Walk& w, Segment& e) {
   if (w.left <= 0) return false;
   const bool one = w.shp.single && w.r == w.shp.pairs - 1;
   const int steps = one ? (w.shp.tiles + 1) >> 1 : w.shp.tiles;
@@ -178,21 +352,23 @@ __device__ __forceinline__ bool walk_next(const Params& p, Walk& w, Segment& e) 
   e.tiles = one ? min(2 * n, w.shp.tiles - e.tile0) : n;
   e.keys = w.grp.keys;
   e.row0 = part_row(p, w.grp, w.h, w.r, blockIdx.x);
+  e.begin = w.s == 0;
+  e.end = w.s + n == steps;
   w.left -= n;
   w.s += n;
   if (w.s == steps && w.left > 0) {
     w.s = 0;
     if (++w.r == w.shp.pairs) {
       w.r = 0;
-      if (++w.h == p.hkv) {
+      if (++w.h == p.own.hkv) {
         w.h = 0;
         int g = w.g;
         do {
-          if (++g >= p.groups.n) {  // groups changed under the kernel
+          if (++g >= p.own.groups.n) {  // groups changed under the kernel
             w.left = 0;
             return true;
           }
-          walk_group(p, w, g);
+          walk_group(p, tab, w, g);
         } while (w.grp.keys == 0);
       }
     }
@@ -207,7 +383,7 @@ __device__ __forceinline__ int tiles_of(const Segment& e, int t) { return e.two 
 // Query rows of tile t, and its first partial row.
 __device__ __forceinline__ int rows_of(const Params& p, const Segment& e, int t) {
   const int seqs = e.two && t ? e.rows - p.per_tile : min(e.rows, p.per_tile);
-  return seqs * p.group;
+  return seqs * p.own.group;
 }
 
 __device__ __forceinline__ uint64_t desc_kmajor(const uint8_t* tile) {
@@ -224,51 +400,494 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// The barriers of the shared part.
+struct Bars {
+  uint64_t* b;
+  __device__ __forceinline__ uint64_t* q_full() const { return b + 0; }    // a segment's Q landed
+  __device__ __forceinline__ uint64_t* q_empty() const { return b + 1; }   // its last S done
+  __device__ __forceinline__ uint64_t* kv_full() const { return b + 2; }   // [kStages]
+  __device__ __forceinline__ uint64_t* kv_empty() const { return b + 6; }  // [kStages]
+  __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2] S_t written
+  __device__ __forceinline__ uint64_t* s_free() const { return b + 12; }   // [2] P_t V done
+  __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2] P_t written (128 arrivals)
+  __device__ __forceinline__ uint64_t* o_empty() const { return b + 16; }  // [2] O_t read by the storing warps (128)
+  __device__ __forceinline__ uint64_t* st_full() const { return b + 18; }  // [2] row sums and maxima of tile t written (128)
+  __device__ __forceinline__ uint64_t* st_empty() const { return b + 20; } // [2] ... and read (128)
+};
+
+__device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.own.err, LA_DEVERR_WAIT_TIMEOUT));
+}
+
+// Softmax of tile t, four warps, a thread per row.
+__device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
+                                             Bars bars, uint32_t tmem, int t, int warp, int lane) {
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
+  uint64_t* s_full = bars.s_full();
+  uint64_t* p_full = bars.p_full();
+  uint64_t* st_full = bars.st_full();
+  uint64_t* st_empty = bars.st_empty();
+  const float NEG_INF = -__int_as_float(0x7f800000);
+  float* stats = reinterpret_cast<float*>(smem + kOffStats);  // [tile][l | m][128]
+  const int quarter = warp & 3;
+  const int row = quarter * 32 + lane;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t colS = t * 128, colO = kColO + t * 128;
+  const float sl2 = p.own.scale_log2;
+  Walk& w = *reinterpret_cast<Walk*>(smem + kOffWalk + warp * kWalkBytes);
+  Segment& e = *reinterpret_cast<Segment*>(smem + kOffWalk + warp * kWalkBytes + 64);
+  {
+    Walk x;
+    walk_start(p, tab, plan, x);
+    if (lane == 0) w = x;
+    __syncwarp();
+  }
+  auto next = [&]() -> bool {
+    Walk x = w;
+    Segment y{};
+    const bool more = walk_next(p, tab, x, y);
+    __syncwarp();  // every lane has read the old state
+    if (lane == 0) {
+      w = x;
+      e = y;
+    }
+    __syncwarp();
+    return more;
+  };
+  uint32_t seen = 0, nst = 0;  // S tiles, segments with statistics
+  bool ok = true;
+  while (ok && next()) {
+    const int n = tiles_of(e, t);
+    if (n == 0) continue;
+    const bool active = quarter * 32 < rows_of(p, e, t);  // rows of this warp
+    float m = NEG_INF, l = 0.f;
+    for (int j = 0; j < n; ++j, ++seen) {
+      if (!(ok = wait_all(&s_full[t], seen & 1))) break;
+      if (!active) {
+        mbar_arrive(&p_full[t]);
+        continue;
+      }
+      tc_fence_after();
+      float sv[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(taddr + colS + c * 32, sv[c]);
+      tc_wait_ld();
+      // keys of this tile, 128 but for the prefix's last
+      const int nvis = e.keys - (e.tile0 + (e.two ? j : 2 * j + t)) * kKeys;
+      float mx[8];
+#pragma unroll
+      for (int a = 0; a < 8; ++a) mx[a] = NEG_INF;
+      if (nvis >= kKeys) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) mx[(x >> 1) & 7] = fmax3(mx[(x >> 1) & 7], sv[c][x], sv[c][x + 1]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            const float x0 = (c * 32 + x < nvis) ? sv[c][x] : NEG_INF;
+            const float x1 = (c * 32 + x + 1 < nvis) ? sv[c][x + 1] : NEG_INF;
+            sv[c][x] = x0;
+            sv[c][x + 1] = x1;
+            mx[(x >> 1) & 7] = fmax3(mx[(x >> 1) & 7], x0, x1);
+          }
+      }
+      const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(fmax3(mx[3], mx[4], mx[5]), mx[6], mx[7])) * sl2;
+      // The reference rises only by more than 2^8 (P stays below that, l
+      // far below overflow), so that O is seldom rescaled.
+      const float m_new = (mt > m + 8.f) ? mt : m;
+      const float m_ref = (m_new == NEG_INF) ? 0.f : m_new;
+      const float alpha = ex2(m - m_ref);
+      const uint64_t sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
+      uint64_t acc2[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) acc2[a] = 0ull;
+      // P rounded to bf16, the type of V, for the product; l sums it unrounded.
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        float pk[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const uint64_t y2 =
+              f2_fma(f2_pack(sv[2 * c2 + (x >> 4)][(x & 15) * 2], sv[2 * c2 + (x >> 4)][(x & 15) * 2 + 1]), sl2x2, negm2);
+          float e0, e1;
+          f2_unpack(y2, e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
+          pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
+        }
+        tmem_st32(taddr + colS + c2 * 32, pk);
+      }
+      float ps[8];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) f2_unpack(acc2[a], ps[2 * a], ps[2 * a + 1]);
+      l = l * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
+      // O_t holds the products of the tiles before: S_t(j) was issued behind
+      // them, and the next waits for this P.
+      if (j >= 1 && __any_sync(0xffffffffu, m_new != m)) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld32(taddr + colO + c * 32, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] *= alpha;
+          tmem_st32(taddr + colO + c * 32, o);
+        }
+      }
+      m = m_new;
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (!ok) break;
+    if (!(ok = wait_all(&st_empty[t], (nst & 1) ^ 1u))) break;
+    stats[(t * 2 + 0) * kRows + row] = l;
+    stats[(t * 2 + 1) * kRows + row] = m;
+    mbar_arrive(&st_full[t]);
+    ++nst;
+  }
+}
+
+// The segments' results, four warps.
+__device__ __forceinline__ void store_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
+                                           Bars bars, uint32_t tmem, int warp, int lane) {
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
+  uint64_t* s_free = bars.s_free();
+  uint64_t* o_empty = bars.o_empty();
+  uint64_t* st_full = bars.st_full();
+  uint64_t* st_empty = bars.st_empty();
+  const float NEG_INF = -__int_as_float(0x7f800000);
+  const float* stats = reinterpret_cast<const float*>(smem + kOffStats);
+  const int quarter = warp & 3;
+  const int row = quarter * 32 + lane;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  uint8_t* stage = smem + kOffStage + quarter * kStageBytes;
+  Walk w;
+  Segment e{};
+  walk_start(p, tab, plan, w);
+  uint32_t done[2] = {0, 0};  // products P_t V, this segment's included
+  uint32_t segs[2] = {0, 0};
+  bool ok = true;
+  while (ok && walk_next(p, tab, w, e)) {
+    for (int t = 0; t < 2 && ok; ++t) {
+      const int rows = rows_of(p, e, t);
+      const int n = tiles_of(e, t);
+      const int row0 = e.row0 + t * rows_of(p, e, 0);
+      if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
+        int4* it = p.items + static_cast<long long>(e.first + t * p.per_tile + row / p.own.group) * p.own.hkv + e.h;
+        if (e.begin) {
+          it->x = row0 + row;
+          it->y = e.two ? 0 : rows;
+          it->z = static_cast<int>(blockIdx.x);
+        }
+        if (e.end) it->w = static_cast<int>(blockIdx.x);
+      }
+      if (n == 0) {  // a single key tile: none for the second accumulator
+        if (row < rows) p.part_lse[row0 + row] = NEG_INF;
+        continue;
+      }
+      done[t] += n;
+      if (!(ok = wait_all(&st_full[t], segs[t] & 1))) break;
+      const float l = stats[(t * 2 + 0) * kRows + row];
+      const float m = stats[(t * 2 + 1) * kRows + row];
+      mbar_arrive(&st_empty[t]);
+      if (!(ok = wait_all(&s_free[t], (done[t] - 1) & 1))) break;  // the last product
+      tc_fence_after();
+      ++segs[t];
+      if (quarter * 32 >= rows) {
+        mbar_arrive(&o_empty[t]);
+        continue;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (row < rows) p.part_lse[row0 + row] = l == 0.f ? NEG_INF : m + __log2f(l);
+      // 32 columns at a time through the staging buffer (16-byte chunks
+      // XORed by row), so that a store instruction writes 4 rows of 128 bytes.
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        tmem_ld32(taddr + kColO + t * 128 + c * 32, o);
+        tc_wait_ld();
+        if (c == 3) {
+          tc_fence_before();
+          mbar_arrive(&o_empty[t]);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<float4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
+              make_float4(o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv);
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int r = x * 4 + (lane >> 3), ch = lane & 7;
+          const float4 u = *reinterpret_cast<const float4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+          if (quarter * 32 + r < rows)
+            *reinterpret_cast<float4*>(p.part_o + static_cast<long long>(row0 + quarter * 32 + r) * kD + c * 32 +
+                                       ch * 4) = u;
+        }
+        __syncwarp();
+      }
+    }
+  }
+}
+
+// TMA loads of the shared part, one warp.
+__device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                          const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
+                                          Bars bars, int lane) {
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
+  uint64_t* q_full = bars.q_full();
+  uint64_t* q_empty = bars.q_empty();
+  uint64_t* kv_full = bars.kv_full();
+  uint64_t* kv_empty = bars.kv_empty();
+  uint8_t* sQ = smem + kOffQ;
+  uint8_t* sKV = smem + kOffKV;
+  Walk w;
+  Segment e{};
+  // Per segment Q, then the tiles in the order the products use them:
+  // `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1 for two row
+  // tiles, 2 for the two accumulators of one.
+  walk_start(p, tab, plan, w);
+  int kq = 0;
+  uint32_t pos = 0;  // tiles loaded
+  bool ok = true;
+  // A box per lane: 64 dims of box_keys keys of one page. The page ids of the
+  // segment's boxes are read 32 at a time, the next 32 in advance; V uses the
+  // ids of its K tile, one or two tiles ago.
+  const int boxes = kKeys / p.box_keys, half = lane & 1, box = lane >> 1;
+  const int per_page = p.own.block_size / p.box_keys;  // boxes of a page
+  const int* row_ids = nullptr;
+  int win = -1, ids = 0, next_ids = 0;
+  int k_id = 0, v_id = 0;  // the last K tile's, and the one that the next V tile takes
+  auto read_ids = [&](const Segment& e, int w0) -> int {
+    const int x = w0 * 32 + lane;
+    return x * p.box_keys < e.keys ? __ldg(row_ids + x / per_page) : -1;
+  };
+  auto start = [&](const Segment& e) {
+    row_ids = p.own.block_table + static_cast<long long>(e.table_row) * p.own.bt_stride;
+    win = e.tile0 * boxes >> 5;
+    ids = read_ids(e, win);
+    next_ids = read_ids(e, win + 1);
+  };
+  auto load = [&](const CUtensorMap* tm, const Segment& e, int tile, int id) -> bool {
+    const int st = pos % kStages;
+    if (!wait_all(&kv_empty[st], ((pos / kStages) & 1) ^ 1u)) return false;
+    uint8_t* dst = sKV + st * kTile;
+    if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTile);
+    __syncwarp();
+    if (box < boxes) {
+      // keys behind the prefix, and pages outside the pool, come from block
+      // num_blocks, outside the tensor map: zeros
+      const int x = tile * boxes + box;
+      const bool in = x * p.box_keys < e.keys;
+      const bool sound = id >= 0 && id < p.own.num_blocks;
+      if (in && !sound && p.own.err) atomicCAS(p.own.err, 0, LA_DEVERR_BLOCK_ID);
+      const int blk = in && sound ? id : static_cast<int>(p.own.num_blocks);
+      tma_load_4d(dst + half * kHalf + box * p.box_keys * 128, tm, &kv_full[st], half * 64,
+                  x % per_page * p.box_keys, e.h, blk);
+    }
+    __syncwarp();
+    ++pos;
+    return true;
+  };
+  auto load_k = [&](const Segment& e, int tile) -> bool {
+    const int x = tile * boxes;
+    if (x >> 5 != win) {
+      win = x >> 5;
+      ids = next_ids;
+      next_ids = read_ids(e, win + 1);
+    }
+    v_id = k_id;
+    k_id = __shfl_sync(0xffffffffu, ids, (x & 31) + min(box, boxes - 1));
+    return load(&tm_k, e, tile, k_id);
+  };
+  while (ok && walk_next(p, tab, w, e)) {
+    start(e);
+    if (!(ok = wait_all(q_empty, (kq & 1) ^ 1u))) break;
+    if (lane == 0) {
+      const uint32_t half = 128u * p.own.group * p.per_tile;
+      mbar_arrive_expect_tx(q_full, (1 + e.two) * 2 * half);
+      for (int t = 0; t < 1 + e.two; ++t)
+        for (int x = 0; x < 2; ++x)
+          tma_load_3d(sQ + t * kTile + x * kHalf, &tm_q, q_full, x * 64, e.h * p.own.group, e.first + t * p.per_tile);
+    }
+    __syncwarp();
+    ++kq;
+    const int lead = 2 - e.two;
+    for (int i = 0; ok && i < min(lead, e.tiles); ++i) ok = load_k(e, e.tile0 + i);
+    for (int i = 0; ok && i < e.tiles; ++i) {
+      // the K tile before last where one more is already loaded
+      ok = load(&tm_v, e, e.tile0 + i, lead == 2 && i + 1 < e.tiles ? v_id : k_id);
+      if (ok && i + lead < e.tiles) ok = load_k(e, e.tile0 + i + lead);
+    }
+  }
+  if (!ok && lane == 0) {  // early exit: let the copies already issued land (bounded)
+    for (uint32_t u = (pos > kStages ? pos - kStages : 0); u < pos; ++u)
+      mbar_wait(&kv_full[u % kStages], (u / kStages) & 1, nullptr, 0);
+    if (kq > 0) mbar_wait(q_full, (kq - 1) & 1, nullptr, 0);
+  }
+  __syncwarp();
+}
+
+// Products of the shared part, one warp; lane 0 issues.
+__device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
+                                             Bars bars, uint32_t tmem, int lane) {
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
+  uint64_t* q_full = bars.q_full();
+  uint64_t* q_empty = bars.q_empty();
+  uint64_t* kv_full = bars.kv_full();
+  uint64_t* kv_empty = bars.kv_empty();
+  uint64_t* s_full = bars.s_full();
+  uint64_t* s_free = bars.s_free();
+  uint64_t* p_full = bars.p_full();
+  uint64_t* o_empty = bars.o_empty();
+  uint8_t* sQ = smem + kOffQ;
+  uint8_t* sKV = smem + kOffKV;
+  Walk w;
+  Segment e{};
+  // S_t over P_t is issued right behind the product that reads P_t: the
+  // tensor core executes one thread's products in order.
+  walk_start(p, tab, plan, w);
+  int kq = 0;
+  uint32_t pos = 0;
+  uint32_t cp[2] = {0, 0}, segs[2] = {0, 0};
+  bool ok = true;
+  auto wait_full = [&](uint32_t x) -> bool { return wait_all(&kv_full[x % kStages], (x / kStages) & 1); };
+  auto issue_s = [&](int t, int q, uint32_t x) {
+    if (lane == 0) {
+      const uint64_t ad = desc_kmajor(sQ + q * kTile), bd = desc_kmajor(sKV + (x % kStages) * kTile);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const int o = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+        umma_f16_ss(tmem + t * 128, ad + o, bd + o, kIdescQK, ks > 0 ? 1u : 0u);
+      }
+      umma_commit(&s_full[t]);
+    }
+    __syncwarp();
+  };
+  auto issue_pv = [&](int t, bool first, uint32_t x) -> bool {
+    if (!wait_all(&p_full[t], cp[t] & 1)) return false;
+    if (first) {  // O_t is overwritten: the previous segment's must have been read
+      if (segs[t] > 0 && !wait_all(&o_empty[t], (segs[t] - 1) & 1)) return false;
+      ++segs[t];
+    }
+    tc_fence_after();
+    if (lane == 0) {
+      const uint64_t vd = desc_v(sKV + (x % kStages) * kTile);
+#pragma unroll
+      for (int ks = 0; ks < kKeys / 16; ++ks)
+        umma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + ks * 8, vd + ks * 128, kIdescPV,
+                    (!first || ks > 0) ? 1u : 0u);
+      umma_commit(&s_free[t]);
+    }
+    __syncwarp();
+    ++cp[t];
+    return true;
+  };
+  auto release = [&](uint64_t* bar) {
+    if (lane == 0) umma_commit(bar);
+    __syncwarp();
+  };
+  while (ok && walk_next(p, tab, w, e)) {
+    if (!(ok = wait_all(q_full, kq & 1))) break;
+    ++kq;
+    const int n = e.tiles, lead = 2 - e.two;
+    for (int i = 0; ok && i < min(lead, n); ++i, ++pos) {
+      if (!(ok = wait_full(pos))) break;
+      if (e.two) {
+        issue_s(0, 0, pos);
+        issue_s(1, 1, pos);
+      } else {
+        issue_s(i, 0, pos);
+      }
+      release(&kv_empty[pos % kStages]);
+    }
+    if (!ok) break;
+    if (n <= lead) release(q_empty);
+    for (int i = 0; ok && i < n; ++i) {
+      const uint32_t vp = pos++;
+      const bool more = i + lead < n;
+      const uint32_t kp = pos;
+      if (more) ++pos;
+      if (!(ok = wait_full(vp))) break;
+      if (more && !(ok = wait_full(kp))) break;
+      if (e.two) {
+        if (!(ok = issue_pv(0, i == 0, vp))) break;
+        if (more) issue_s(0, 0, kp);
+        if (!(ok = issue_pv(1, i == 0, vp))) break;
+        release(&kv_empty[vp % kStages]);
+        if (more) issue_s(1, 1, kp);
+      } else {
+        if (!(ok = issue_pv(i & 1, i < 2, vp))) break;
+        release(&kv_empty[vp % kStages]);
+        if (more) issue_s(i & 1, 0, kp);
+      }
+      if (more) release(&kv_empty[kp % kStages]);
+      if (more && i + 1 + lead == n) release(q_empty);  // the segment's last S
+    }
+  }
+  __syncwarp();
+}
+
+// What the combine pass has to read of each row, one warp.
+__device__ __forceinline__ void write_flags(const Params& p, const PrefixGroup* tab, int lane) {
+  for (int b = lane; b < p.own.batch; b += 32) {
+    int block0;
+    const int own = decode::own_keys<true>(p.own, tab, b, &block0);
+    p.flags[b] = (block0 > 0 ? kShares : 0) | (own > 0 ? kOwn : 0);
+  }
+}
+
+// kOwnStages: pipeline stages of the decode warps.
+template <int kOwnStages>
 __global__ void __launch_bounds__(kThreads, 1)
-    prefix_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                  const __grid_constant__ CUtensorMap tm_v, const Params p) {
+    shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap own_q,
+                         const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
+                         const __grid_constant__ CUtensorMap own_k1, const __grid_constant__ CUtensorMap own_v1,
+                         const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;
-  uint8_t* sKV = smem + kOffKV;
-  float* stats = reinterpret_cast<float*>(smem + kOffStats);  // [tile][l | m][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint64_t* q_full = bars + 0;     // a segment's Q landed
-  uint64_t* q_empty = bars + 1;    // its last S done
-  uint64_t* kv_full = bars + 2;    // [kStages]
-  uint64_t* kv_empty = bars + 6;   // [kStages]
-  uint64_t* s_full = bars + 10;    // [2] S_t written
-  uint64_t* s_free = bars + 12;    // [2] P_t V done
-  uint64_t* p_full = bars + 14;    // [2] P_t written (128 arrivals)
-  uint64_t* o_empty = bars + 16;   // [2] O_t read by the storing warps (128)
-  uint64_t* st_full = bars + 18;   // [2] row sums and maxima of tile t written (128)
-  uint64_t* st_empty = bars + 20;  // [2] ... and read (128)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
-  Range* range = reinterpret_cast<Range*>(bars + 24);
-
+  const Bars bars{reinterpret_cast<uint64_t*>(smem)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 192);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffOwnBar);
+  uint64_t* empty = full + decode::kMaxStages;
+  uint64_t* mg_full = empty + decode::kMaxStages;  // all consumer warps wrote their state
+  uint64_t* mg_empty = mg_full + 1;                // the merging warp read it
+  PrefixGroup* tab = p.own.groups.n <= kMaxGroups ? reinterpret_cast<PrefixGroup*>(smem + kOffTable) : nullptr;
+  Plan& plan = *reinterpret_cast<Plan*>(smem + kOffPlan);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int wg = warp >> 2;
-  const float NEG_INF = -__int_as_float(0x7f800000);
 
   // Barriers and tensor memory: nothing that a kernel before this one writes.
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+  if (threadIdx.x == 32) {
+    mbar_init(bars.q_full(), 1);
+    mbar_init(bars.q_empty(), 1);
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(bars.kv_full() + i, 1);
+      mbar_init(bars.kv_empty() + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_empty[i], 128);
-      mbar_init(&st_full[i], 128);
-      mbar_init(&st_empty[i], 128);
+      mbar_init(bars.s_full() + i, 1);
+      mbar_init(bars.s_free() + i, 1);
+      mbar_init(bars.p_full() + i, 128);
+      mbar_init(bars.o_empty() + i, 128);
+      mbar_init(bars.st_full() + i, 128);
+      mbar_init(bars.st_empty() + i, 128);
     }
+    for (int s = 0; s < kOwnStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], decode::kCWarps);
+    }
+    mbar_init(mg_full, decode::kCWarps);
+    mbar_init(mg_empty, p.own.hkv);
     fence_barrier_init();
   }
+  if (warp == 2) reinterpret_cast<uint32_t*>(smem + kOffZero)[lane] = 0u;
   if (warp == 12) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
@@ -277,403 +896,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&own_q);
+    tma_prefetch_desc(&own_k);
+    tma_prefetch_desc(&own_v);
   }
   grid_dependency_wait();
-  // What came before is done and visible, so the row-by-row pass behind this
-  // grid may start wherever an SM is free: it reads nothing written here.
-  grid_launch_dependents();
-  if (warp == 14) {
-    // all steps, then the group that holds the CTA's first one
-    const int n = p.groups.n;
-    long long T = 0;
-    for (int b = 0; b < n; b += 32) {
-      const int g = b + lane;
-      if (blockIdx.x == 0 && g < n && p.err) {
-        const int lo = p.groups.cu[g], hi = p.groups.cu[g + 1];
-        if (lo < 0 || hi < lo || hi > p.groups.batch) atomicCAS(p.err, 0, LA_DEVERR_PREFIX);
-      }
-      long long s = g < n ? steps_of(p, g) : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      T += s;
-    }
-    const long long G = parts_of(T, gridDim.x);
-    const long long u0 = blockIdx.x < G ? part_start(blockIdx.x, T, G) : T;
-    const long long u1 = blockIdx.x < G ? part_start(blockIdx.x + 1, T, G) : T;
-    long long acc = 0, before = 0;
-    int g0 = 0;
-    for (int b = 0; u0 < u1 && b < n; b += 32) {
-      const int g = b + lane;
-      const int s = g < n ? steps_of(p, g) : 0;
-      long long incl = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > u0);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        g0 = b + src;
-        before = acc + __shfl_sync(0xffffffffu, incl - s, src);
-        break;
-      }
-      acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (lane == 0) *range = Range{u0, u1, before, g0};
+  grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
+  if (warp == 0) {
+    const Plan r = make_plan(p, tab, lane);
+    if (lane == 0) plan = r;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (range->u0 >= range->u1) {  // no work
-    if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+  const int P = plan.P;
+  const bool shares = static_cast<int>(blockIdx.x) < P;
+  if (warp == 12 && !shares) tmem_dealloc(tmem, kTmemCols);
+  if (!shares) {
+    if (wg < 2) {
+      regs_inc<kRegConsume>();
+      decode::consume<kOwnStages, true>(p.own, smem + kCtrlBytes, full, empty,
+                                        reinterpret_cast<const decode::StageDesc*>(smem + kOffDesc), smem + kOffZero,
+                                        mg_full, mg_empty,
+                                        reinterpret_cast<float*>(smem + kCtrlBytes + kOwnStages * p.own.stage_bytes),
+                                        plan.u1 - plan.u0, warp, lane);
+    } else if (wg == 2) {
+      regs_dec<kRegLoad>();
+      if (warp < decode::kCWarps + 2 && plan.u1 > plan.u0) {
+        decode::Windows<true> w;
+        w.tab = tab;
+        w.load_swin(p.own, lane, plan.at);
+        w.load_bwin(p.own, lane, plan.at, static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
+        decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
+                                          reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), w, plan.u0,
+                                          plan.u1 - plan.u0, plan.at, plan.before, static_cast<int>(blockIdx.x) - P,
+                                          warp - decode::kCWarps, 2, lane);
+      }
+    } else {
+      regs_dec<kRegIdle>();
+      if (warp == 15 && blockIdx.x == 0) write_flags(p, tab, lane);
+    }
     return;
   }
-
-  auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err, LA_DEVERR_WAIT_TIMEOUT));
-  };
   if (wg < 2) {
     regs_inc<kRegSoftmax>();
-    // ------------------------------------------------------------ softmax of tile t
-    const int t = wg;
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t colS = t * 128, colO = kColO + t * 128;
-    const float sl2 = p.scale_log2;
-    Walk& w = *reinterpret_cast<Walk*>(smem + kOffWalk + warp * kWalkBytes);
-    Segment& e = *reinterpret_cast<Segment*>(smem + kOffWalk + warp * kWalkBytes + 64);
-    {
-      Walk x;
-      walk_start(p, *range, x);
-      if (lane == 0) w = x;
-      __syncwarp();
-    }
-    auto next = [&]() -> bool {
-      Walk x = w;
-      Segment y{};
-      const bool more = walk_next(p, x, y);
-      __syncwarp();  // every lane has read the old state
-      if (lane == 0) {
-        w = x;
-        e = y;
-      }
-      __syncwarp();
-      return more;
-    };
-    uint32_t seen = 0, nst = 0;  // S tiles, segments with statistics
-    bool ok = true;
-    while (ok && next()) {
-      const int n = tiles_of(e, t);
-      if (n == 0) continue;
-      const bool active = quarter * 32 < rows_of(p, e, t);  // rows of this warp
-      float m = NEG_INF, l = 0.f;
-      for (int j = 0; j < n; ++j, ++seen) {
-        if (!(ok = wait_all(&s_full[t], seen & 1))) break;
-        if (!active) {
-          mbar_arrive(&p_full[t]);
-          continue;
-        }
-        tc_fence_after();
-        float sv[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(taddr + colS + c * 32, sv[c]);
-        tc_wait_ld();
-        // keys of this tile, 128 but for the prefix's last
-        const int nvis = e.keys - (e.tile0 + (e.two ? j : 2 * j + t)) * kKeys;
-        float mx[8];
-#pragma unroll
-        for (int a = 0; a < 8; ++a) mx[a] = NEG_INF;
-        if (nvis >= kKeys) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) mx[(x >> 1) & 7] = fmax3(mx[(x >> 1) & 7], sv[c][x], sv[c][x + 1]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const float x0 = (c * 32 + x < nvis) ? sv[c][x] : NEG_INF;
-              const float x1 = (c * 32 + x + 1 < nvis) ? sv[c][x + 1] : NEG_INF;
-              sv[c][x] = x0;
-              sv[c][x + 1] = x1;
-              mx[(x >> 1) & 7] = fmax3(mx[(x >> 1) & 7], x0, x1);
-            }
-        }
-        const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(fmax3(mx[3], mx[4], mx[5]), mx[6], mx[7])) * sl2;
-        // The reference rises only by more than 2^8 (P stays below that, l
-        // far below overflow), so that O is seldom rescaled.
-        const float m_new = (mt > m + 8.f) ? mt : m;
-        const float m_ref = (m_new == NEG_INF) ? 0.f : m_new;
-        const float alpha = ex2(m - m_ref);
-        const uint64_t sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
-        uint64_t acc2[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) acc2[a] = 0ull;
-        // P rounded to bf16, the type of V, for the product; l sums it unrounded.
-#pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
-          float pk[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const uint64_t y2 =
-                f2_fma(f2_pack(sv[2 * c2 + (x >> 4)][(x & 15) * 2], sv[2 * c2 + (x >> 4)][(x & 15) * 2 + 1]), sl2x2, negm2);
-            float e0, e1;
-            f2_unpack(y2, e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
-            pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
-          }
-          tmem_st32(taddr + colS + c2 * 32, pk);
-        }
-        float ps[8];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) f2_unpack(acc2[a], ps[2 * a], ps[2 * a + 1]);
-        l = l * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
-        // O_t holds the products of the tiles before: S_t(j) was issued behind
-        // them, and the next waits for this P.
-        if (j >= 1 && __any_sync(0xffffffffu, m_new != m)) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float o[32];
-            tmem_ld32(taddr + colO + c * 32, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] *= alpha;
-            tmem_st32(taddr + colO + c * 32, o);
-          }
-        }
-        m = m_new;
-        tc_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
-      }
-      if (!ok) break;
-      if (!(ok = wait_all(&st_empty[t], (nst & 1) ^ 1u))) break;
-      stats[(t * 2 + 0) * kRows + row] = l;
-      stats[(t * 2 + 1) * kRows + row] = m;
-      mbar_arrive(&st_full[t]);
-      ++nst;
-    }
+    softmax_warp(p, tab, plan, smem, bars, tmem, wg, warp, lane);
   } else if (wg == 2) {
     regs_dec<kRegStore>();
-    // ------------------------------------------------------------ segments' results
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint8_t* stage = smem + kOffStage + quarter * kStageBytes;
-    Walk w;
-    Segment e{};
-    walk_start(p, *range, w);
-    uint32_t done[2] = {0, 0};  // products P_t V, this segment's included
-    uint32_t segs[2] = {0, 0};
-    bool ok = true;
-    while (ok && walk_next(p, w, e)) {
-      for (int t = 0; t < 2 && ok; ++t) {
-        const int rows = rows_of(p, e, t);
-        const int n = tiles_of(e, t);
-        const int row0 = e.row0 + t * rows_of(p, e, 0);
-        if (n == 0) {  // a single key tile: none for the second accumulator
-          if (row < rows) p.part_lse[row0 + row] = NEG_INF;
-          continue;
-        }
-        done[t] += n;
-        if (!(ok = wait_all(&st_full[t], segs[t] & 1))) break;
-        const float l = stats[(t * 2 + 0) * kRows + row];
-        const float m = stats[(t * 2 + 1) * kRows + row];
-        mbar_arrive(&st_empty[t]);
-        if (!(ok = wait_all(&s_free[t], (done[t] - 1) & 1))) break;  // the last product
-        tc_fence_after();
-        ++segs[t];
-        if (quarter * 32 >= rows) {
-          mbar_arrive(&o_empty[t]);
-          continue;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (row < rows) p.part_lse[row0 + row] = l == 0.f ? NEG_INF : m + __log2f(l);
-        // 32 columns at a time through the staging buffer (16-byte chunks
-        // XORed by row), so that a store instruction writes 4 rows of 128 bytes.
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          tmem_ld32(taddr + kColO + t * 128 + c * 32, o);
-          tc_wait_ld();
-          if (c == 3) {
-            tc_fence_before();
-            mbar_arrive(&o_empty[t]);
-          }
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-                make_float4(o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv);
-          __syncwarp();
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int r = x * 4 + (lane >> 3), ch = lane & 7;
-            const float4 u = *reinterpret_cast<const float4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
-            if (quarter * 32 + r < rows)
-              *reinterpret_cast<float4*>(p.part_o + static_cast<long long>(row0 + quarter * 32 + r) * kD + c * 32 +
-                                         ch * 4) = u;
-          }
-          __syncwarp();
-        }
-      }
-    }
+    store_warp(p, tab, plan, smem, bars, tmem, warp, lane);
   } else {
     regs_dec<kRegOther>();
-    Walk w;
-    Segment e{};
-    if (warp == 13) {
-      // ---------------------------------------------------------- TMA producer
-      // Per segment Q, then the tiles in the order the products use them:
-      // `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1 for two row
-      // tiles, 2 for the two accumulators of one.
-      walk_start(p, *range, w);
-      int kq = 0;
-      uint32_t pos = 0;  // tiles loaded
-      bool ok = true;
-      const int boxes = kKeys / p.box_keys;
-      auto load = [&](const CUtensorMap* tm, int tile) -> bool {
-        const int st = pos % kStages;
-        if (!wait_all(&kv_empty[st], ((pos / kStages) & 1) ^ 1u)) return false;
-        uint8_t* dst = sKV + st * kTile;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTile);
-        __syncwarp();
-        if (lane < 2 * boxes) {  // a box per lane: 64 dims of box_keys keys of one page
-          const int key = tile * kKeys + (lane >> 1) * p.box_keys;
-          // keys behind the prefix, and pages outside the pool, come from
-          // block num_blocks, outside the tensor map: zeros
-          int blk = p.num_blocks, off = 0;
-          if (key < e.keys) {
-            const int lb = p.groups.bs_shift >= 0 ? key >> p.groups.bs_shift : key / p.groups.block_size;
-            off = key - lb * p.groups.block_size;
-            const int id = __ldg(p.table + static_cast<long long>(e.table_row) * p.table_stride + lb);
-            if (id >= 0 && id < p.num_blocks)
-              blk = id;
-            else if (p.err)
-              atomicCAS(p.err, 0, LA_DEVERR_BLOCK_ID);
-          }
-          tma_load_4d(dst + (lane & 1) * kHalf + (lane >> 1) * p.box_keys * 128, tm, &kv_full[st], (lane & 1) * 64, off,
-                      e.h, blk);
-        }
-        __syncwarp();
-        ++pos;
-        return true;
-      };
-      while (ok && walk_next(p, w, e)) {
-        if (!(ok = wait_all(q_empty, (kq & 1) ^ 1u))) break;
-        if (lane == 0) {
-          const uint32_t half = 128u * p.group * p.per_tile;
-          mbar_arrive_expect_tx(q_full, (1 + e.two) * 2 * half);
-          for (int t = 0; t < 1 + e.two; ++t)
-            for (int x = 0; x < 2; ++x)
-              tma_load_3d(sQ + t * kTile + x * kHalf, &tm_q, q_full, x * 64, e.h * p.group, e.first + t * p.per_tile);
-        }
-        __syncwarp();
-        ++kq;
-        const int lead = 2 - e.two;
-        for (int i = 0; ok && i < min(lead, e.tiles); ++i) ok = load(&tm_k, e.tile0 + i);
-        for (int i = 0; ok && i < e.tiles; ++i) {
-          ok = load(&tm_v, e.tile0 + i);
-          if (ok && i + lead < e.tiles) ok = load(&tm_k, e.tile0 + i + lead);
-        }
-      }
-      if (!ok && lane == 0) {  // early exit: let the copies already issued land (bounded)
-        for (uint32_t u = (pos > kStages ? pos - kStages : 0); u < pos; ++u)
-          mbar_wait(&kv_full[u % kStages], (u / kStages) & 1, nullptr, 0);
-        if (kq > 0) mbar_wait(q_full, (kq - 1) & 1, nullptr, 0);
-      }
-      __syncwarp();
-    } else if (warp == 12) {
-      // ---------------------------------------------------------- products (lane 0 issues)
-      // S_t over P_t is issued right behind the product that reads P_t: the
-      // tensor core executes one thread's products in order.
-      walk_start(p, *range, w);
-      int kq = 0;
-      uint32_t pos = 0;
-      uint32_t cp[2] = {0, 0}, segs[2] = {0, 0};
-      bool ok = true;
-      auto wait_full = [&](uint32_t x) -> bool { return wait_all(&kv_full[x % kStages], (x / kStages) & 1); };
-      auto issue_s = [&](int t, int q, uint32_t x) {
-        if (lane == 0) {
-          const uint64_t ad = desc_kmajor(sQ + q * kTile), bd = desc_kmajor(sKV + (x % kStages) * kTile);
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const int o = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
-            umma_f16_ss(tmem + t * 128, ad + o, bd + o, kIdescQK, ks > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[t]);
-        }
-        __syncwarp();
-      };
-      auto issue_pv = [&](int t, bool first, uint32_t x) -> bool {
-        if (!wait_all(&p_full[t], cp[t] & 1)) return false;
-        if (first) {  // O_t is overwritten: the previous segment's must have been read
-          if (segs[t] > 0 && !wait_all(&o_empty[t], (segs[t] - 1) & 1)) return false;
-          ++segs[t];
-        }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint64_t vd = desc_v(sKV + (x % kStages) * kTile);
-#pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            umma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + ks * 8, vd + ks * 128, kIdescPV,
-                        (!first || ks > 0) ? 1u : 0u);
-          umma_commit(&s_free[t]);
-        }
-        __syncwarp();
-        ++cp[t];
-        return true;
-      };
-      auto release = [&](uint64_t* bar) {
-        if (lane == 0) umma_commit(bar);
-        __syncwarp();
-      };
-      while (ok && walk_next(p, w, e)) {
-        if (!(ok = wait_all(q_full, kq & 1))) break;
-        ++kq;
-        const int n = e.tiles, lead = 2 - e.two;
-        for (int i = 0; ok && i < min(lead, n); ++i, ++pos) {
-          if (!(ok = wait_full(pos))) break;
-          if (e.two) {
-            issue_s(0, 0, pos);
-            issue_s(1, 1, pos);
-          } else {
-            issue_s(i, 0, pos);
-          }
-          release(&kv_empty[pos % kStages]);
-        }
-        if (!ok) break;
-        if (n <= lead) release(q_empty);
-        for (int i = 0; ok && i < n; ++i) {
-          const uint32_t vp = pos++;
-          const bool more = i + lead < n;
-          const uint32_t kp = pos;
-          if (more) ++pos;
-          if (!(ok = wait_full(vp))) break;
-          if (more && !(ok = wait_full(kp))) break;
-          if (e.two) {
-            if (!(ok = issue_pv(0, i == 0, vp))) break;
-            if (more) issue_s(0, 0, kp);
-            if (!(ok = issue_pv(1, i == 0, vp))) break;
-            release(&kv_empty[vp % kStages]);
-            if (more) issue_s(1, 1, kp);
-          } else {
-            if (!(ok = issue_pv(i & 1, i < 2, vp))) break;
-            release(&kv_empty[vp % kStages]);
-            if (more) issue_s(i & 1, 0, kp);
-          }
-          if (more) release(&kv_empty[kp % kStages]);
-          if (more && i + 1 + lead == n) release(q_empty);  // the segment's last S
-        }
-      }
-      __syncwarp();
-    }
-    // warps 14, 15: no role
+    if (warp == 12) product_warp(p, tab, plan, smem, bars, tmem, lane);
+    if (warp == 15 && blockIdx.x == 0) write_flags(p, tab, lane);
+    if (warp == 13) load_warp(tm_q, tm_k, tm_v, p, tab, plan, smem, bars, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -684,23 +960,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ combine
-// A CTA per row, a warp per query head (heads behind the 16th in turn), lane l
-// owning dims 4l..4l+3. The row's parts are those of its group's item, one per
-// CTA that had a segment of it (two where the accumulators took alternate key
-// tiles), and those of its own keys. Up to 32 parts per round, one per lane:
-// the weights come from a warp maximum, then the O rows are read 16 at a time.
-// Where they lie follows from the lengths and groups, which are final long
-// before the parts are, so it is worked out before the wait for them.
+// A warp per (row, query head), lane l owning dims 4l..4l+3. The row's parts
+// are those of its group's item, one per CTA that had a segment of it (two
+// where the accumulators took alternate key tiles), and those of its own
+// keys. Up to 32 parts per round, one per lane: the weights come from a warp
+// maximum, the O rows are read 16 at a time, the first 16 together with the
+// logarithms. Bound by the latency of its three dependent reads.
 constexpr int kCombineBatch = 16;
-constexpr int kCombineWarps = 16;
+constexpr int kCombineWarps = 4;
 
 struct CombineParams {
-  PrefixGroups groups;
-  const int* seqlens;
-  int hq, hkv, group, per_tile;
-  int grid;   // CTAs of both passes
-  int tc;     // keys per unit of the row-by-row pass
-  int own0;   // its first partial row
+  const int* flags;
+  const int2* row_parts;
+  const int4* items;
+  int hq, hkv, group;
+  int grid;   // CTAs that parts come from, at most
+  int own0;   // first partial row of the rows' own keys
+  int rows;   // all partial rows
   const float* part_o;
   const float* part_lse;
   __nv_bfloat16* out;
@@ -708,177 +984,126 @@ struct CombineParams {
   float* lse;
 };
 
-__device__ __forceinline__ int clamp_ctx(const CombineParams& p, int b) {
-  const long long c = max(p.seqlens[b], 0);
-  return static_cast<int>(c > p.groups.cap ? p.groups.cap : c);
-}
-
 __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const CombineParams p) {
-  __shared__ long long red[2][kCombineWarps];
-  __shared__ long long steps[2];
   const int b = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int hh = blockIdx.y * static_cast<int>(blockDim.x >> 5) + static_cast<int>(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
   const float NEG_INF = -__int_as_float(0x7f800000);
-
-  // All units, and those before this row.
-  long long T = 0, before = 0;
-  for (int x = threadIdx.x; x < p.groups.batch; x += blockDim.x) {
-    const int ctx = clamp_ctx(p, x);
-    const int n = ctx > 0 ? (ctx - prefix_keys(p.groups, x, ctx) + p.tc - 1) / p.tc : 0;
-    T += n;
-    if (x < b) before += n;
-  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (hh >= p.hq) return;
+  const int h = hh / p.group;
+  const int flags = p.flags[b];
+  const int2 rp = p.row_parts[b];
+  const int4 it = p.items[static_cast<long long>(b) * p.hkv + h];
+  // Groups that are reported as unsound leave entries unwritten: whatever they
+  // hold, the reads below stay inside the workspace.
+  int pn = 0, own = 0;
+  if (flags & kShares) pn = max(0, min(it.w - it.z + 1, p.grid)) * (it.y ? 2 : 1);
+  if (flags & kOwn) own = max(0, min(rp.y - rp.x + 1, p.grid));
+  if (!(flags & kShares) && own == 1) return;  // written by the CTA that read the row
+  const int n = pn + own;
+  float m = NEG_INF, l = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int e0 = 0; e0 < n; e0 += 32) {
+    const int x = e0 + lane;
+    int row = 0;
+    if (x < pn)
+      row = it.x + hh - h * p.group + (it.y ? (x >> 1) * 2 * kRows + (x & 1) * it.y : x * 2 * kRows);
+    else if (x < n)
+      row = p.own0 + (b + rp.x + x - pn) * p.hq + hh;
+    row = min(max(row, 0), p.rows - 1);
+    const float ls = x < n ? p.part_lse[row] : NEG_INF;
+    const int nr = min(n - e0, 32);
+    int su[kCombineBatch];
+    float4 ov[kCombineBatch];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    T += __shfl_xor_sync(0xffffffffu, T, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  if (lane == 0) {
-    red[0][warp] = T;
-    red[1][warp] = before;
-  }
-  // All steps, and those before this row's group.
-  const int ctx = clamp_ctx(p, b);
-  const int gi = prefix_group_of(p.groups, b);
-  Params sp;  // what steps_of reads
-  sp.groups = p.groups;
-  sp.hkv = p.hkv;
-  sp.group = p.group;
-  sp.per_tile = p.per_tile;
-  if (warp == 0) {
-    long long s = 0, sb = 0;
-    for (int g = lane; g < p.groups.n; g += 32) {
-      const int n = steps_of(sp, g);
-      s += n;
-      if (g < gi) sb += n;
-    }
+    for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, k);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      sb += __shfl_xor_sync(0xffffffffu, sb, o);
-    }
-    if (lane == 0) {
-      steps[0] = s;
-      steps[1] = sb;
-    }
-  }
-  __syncthreads();
-  T = before = 0;
-  for (int x = 0; x < warps; ++x) {
-    T += red[0][x];
-    before += red[1][x];
-  }
-  const int shared = prefix_keys(p.groups, b, ctx);
-  const int nb = (ctx - shared + p.tc - 1) / p.tc;
-  const long long G = parts_of(T, p.grid);
-  const int cf = nb > 0 ? part_of(before, T, G) : 0;
-  const int own = nb > 0 ? part_of(before + nb - 1, T, G) - cf + 1 : 0;
-
-  for (int hh = warp; hh < p.hq; hh += warps) {
-    // the group's parts: CTAs pf.., `per` each, whose first row is row0
-    int pn = 0, row0 = 0, per = 1, stride = 0;
-    if (shared > 0) {
-      const PrefixGroup g = prefix_group(p.groups, gi);
-      const Shape s = shape_of(g, p.per_tile);
-      const int h = hh / p.group;
-      const int seq = b - g.first, r = seq / (2 * p.per_tile), in = seq - r * 2 * p.per_tile;
-      const bool one = s.single && r == s.pairs - 1;
-      const long long u0 = steps[1] + static_cast<long long>(h) * s.per_head + r * s.tiles;
-      const int n = one ? (s.tiles + 1) >> 1 : s.tiles;
-      const long long PG = parts_of(steps[0], p.grid);
-      const int pf = part_of(u0, steps[0], PG), pl = part_of(u0 + n - 1, steps[0], PG);
-      per = one ? 2 : 1;
-      pn = (pl - pf + 1) * per;
-      // rows of a tile: (sequence, query head of the kv head); the second
-      // tile's, or accumulator's, behind those of the first
-      const int tile = one ? 0 : in / p.per_tile;
-      stride = one ? (g.rows - r * 2 * p.per_tile) * p.group : 0;
-      row0 = part_row(sp, g, h, r, pf) + tile * p.per_tile * p.group + (in - tile * p.per_tile) * p.group + hh % p.group;
-    }
-    if (hh == warp) grid_dependency_wait();
-    const int n = pn + own;
-    __nv_bfloat16* out = p.out + b * p.out_bs + hh * p.out_hs + lane * 4;
-    float* lse = p.lse ? p.lse + static_cast<long long>(b) * p.hq + hh : nullptr;
-    if (shared == 0 && own == 1) continue;  // written by the row-by-row pass
-    float m = NEG_INF, l = 0.f;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int e0 = 0; e0 < n; e0 += 32) {
-      const int x = e0 + lane;
-      int row = -1;
-      if (x < pn)
-        row = per == 2 ? row0 + (x >> 1) * 2 * kRows + (x & 1) * stride : row0 + x * 2 * kRows;
-      else if (x < n)
-        row = p.own0 + (b + cf + x - pn) * p.hq + hh;
-      const float ls = row >= 0 ? p.part_lse[row] : NEG_INF;
-      const int nr = min(n - e0, 32);
-      int su[kCombineBatch];
-      float4 ov[kCombineBatch];
+    for (int k = 0; k < kCombineBatch; ++k)
+      ov[k] = k < nr ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    // A part without keys has -inf and is left out by a test, never by a
+    // weight of 0, so whatever its row holds does not count; NaN counts.
+    const bool use = x < n && ls != NEG_INF;
+    const unsigned usem = __ballot_sync(0xffffffffu, use);
+    if (usem == 0) continue;
+    float mr = use ? ls : NEG_INF;
 #pragma unroll
-      for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, k);
+    for (int o = 16; o > 0; o >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
+    const float mn = fmaxf(m, mr);
+    const float a = ex2(m - mn);
+    const float wl = use ? ex2(ls - mn) : 0.f;
+    float ws = wl;
 #pragma unroll
-      for (int k = 0; k < kCombineBatch; ++k)
-        ov[k] = k < nr ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-      // A part without keys has -inf and is left out by a test, never by a
-      // weight of 0, so whatever its row holds does not count; NaN counts.
-      const bool use = row >= 0 && ls != NEG_INF;
-      const unsigned usem = __ballot_sync(0xffffffffu, use);
-      if (usem == 0) continue;
-      float mr = use ? ls : NEG_INF;
+    for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+    l = l * a + ws;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
-      const float mn = fmaxf(m, mr);
-      const float a = ex2(m - mn);
-      const float wl = use ? ex2(ls - mn) : 0.f;
-      float ws = wl;
+    for (int k = 0; k < 4; ++k) acc[k] *= a;
+    m = mn;
+#pragma unroll 1
+    for (int j0 = 0; j0 < nr; j0 += kCombineBatch) {
+      if (j0 > 0) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-      l = l * a + ws;
+        for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, (j0 + k) & 31);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] *= a;
-      m = mn;
-      for (int j0 = 0; j0 < nr; j0 += kCombineBatch) {
-        if (j0 > 0) {
+        for (int k = 0; k < kCombineBatch; ++k)
+          ov[k] = j0 + k < nr
+                      ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
-          for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, (j0 + k) & 31);
-#pragma unroll
-          for (int k = 0; k < kCombineBatch; ++k)
-            ov[k] = j0 + k < nr
-                        ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k) {
-          const float wk = __shfl_sync(0xffffffffu, wl, (j0 + k) & 31);
-          if (j0 + k < nr && ((usem >> ((j0 + k) & 31)) & 1u)) {
-            acc[0] += wk * ov[k].x;
-            acc[1] += wk * ov[k].y;
-            acc[2] += wk * ov[k].z;
-            acc[3] += wk * ov[k].w;
-          }
+      for (int k = 0; k < kCombineBatch; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, wl, (j0 + k) & 31);
+        if (j0 + k < nr && ((usem >> ((j0 + k) & 31)) & 1u)) {
+          acc[0] += wk * ov[k].x;
+          acc[1] += wk * ov[k].y;
+          acc[2] += wk * ov[k].z;
+          acc[3] += wk * ov[k].w;
         }
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint2 v;
-    v.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    v.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2*>(out) = v;
-    if (lse && lane == 0) *lse = l == 0.f ? NEG_INF : (m + __log2f(l)) * 0.6931471805599453f;
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint2 v;
+  v.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  v.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<uint2*>(p.out + b * p.out_bs + hh * p.out_hs + lane * 4) = v;
+  if (p.lse && lane == 0)
+    p.lse[static_cast<long long>(b) * p.hq + hh] = l == 0.f ? NEG_INF : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
-// Partial rows: of the prefix pass, then of the row-by-row pass.
-static int64_t prefix_rows(int64_t batch, int hq, int grid) { return 2 * batch * hq + 2 * kRows * grid; }
-static int64_t own_rows(int64_t batch, int hq, int grid) { return (batch + grid) * hq; }
+// The workspace: partial rows of the shared part and of the rows' own keys
+// (O, then logarithms), and what the combine pass reads of each row.
+struct Workspace {
+  int64_t own0, rows;              // partial rows
+  size_t lse, items, parts, flags;  // byte offsets; part_o is at 0
+  size_t bytes;
+};
+
+static Workspace workspace_of(int64_t batch, int hq, int hkv, int64_t grid) {
+  Workspace w;
+  w.own0 = 2 * batch * hq + 2 * kRows * grid;
+  w.rows = w.own0 + (batch + grid) * hq;
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  w.lse = up(static_cast<size_t>(w.rows) * kD * sizeof(float));
+  w.items = up(w.lse + static_cast<size_t>(w.rows) * sizeof(float));
+  w.parts = up(w.items + static_cast<size_t>(batch) * hkv * sizeof(int4));
+  w.flags = up(w.parts + static_cast<size_t>(batch) * sizeof(int2));
+  w.bytes = up(w.flags + static_cast<size_t>(batch) * sizeof(int));
+  return w;
+}
 
 }  // namespace prefix
 
 int prefix_init(int device) {
   (void)device;
-  cudaError_t e = cudaFuncSetAttribute(prefix::prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(prefix::kSmemBytes));
+  const int lim = 227 * 1024;
+  cudaError_t e =
+      cudaFuncSetAttribute(prefix::shared_prefix_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(prefix::shared_prefix_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
   cudaFuncAttributes a;
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, prefix::combine_kernel);
   return cuda_status(e);
@@ -894,9 +1119,9 @@ extern "C" int la_paged_decode_shared_prefix_workspace_size(int device, int batc
     return head_dim != kD ? LA_ERR_UNSUPPORTED : LA_ERR_INVALID_ARGUMENT;
   const int grid = la::num_sms(device);
   if (grid <= 0) return LA_ERR_CUDA;
-  const int64_t rows = prefix_rows(batch, num_q_heads, grid) + own_rows(batch, num_q_heads, grid);
-  if (rows > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
-  *bytes = static_cast<size_t>(rows) * (kD + 1) * sizeof(float) + 256;
+  const Workspace w = workspace_of(batch, num_q_heads, num_kv_heads, grid);
+  if (w.rows > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
+  *bytes = w.bytes;
   return LA_OK;
 }
 
@@ -909,120 +1134,97 @@ extern "C" int la_paged_decode_shared_prefix(
     float* softmax_lse, void* workspace, size_t workspace_bytes, int* dev_error, cudaStream_t stream) {
   using namespace la;
   using namespace la::prefix;
-  if (!q || !k_cache || !v_cache || !block_table || !cache_seqlens || !out ||
-      (num_groups > 0 && (!prefix_lens || !cu_prefix_rows)))
-    return LA_ERR_INVALID_ARGUMENT;
-  if (batch < 0 || num_groups < 0 || num_blocks <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
-    return LA_ERR_INVALID_ARGUMENT;
-  if (batch == 0) return LA_OK;
-  if (head_dim != kD) return LA_ERR_UNSUPPORTED;
-  if (num_kv_heads <= 0 || num_kv_heads > 8 || 8 % num_kv_heads != 0) return LA_ERR_UNSUPPORTED;
-  if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return LA_ERR_INVALID_ARGUMENT;
-  const int group = num_q_heads / num_kv_heads;
-  if (group > 8) return LA_ERR_UNSUPPORTED;
-  if (block_size % 16 != 0 || num_blocks > 0x7ffffffeLL) return LA_ERR_UNSUPPORTED;
-  if (!(softmax_scale > 0.f)) return LA_ERR_INVALID_ARGUMENT;
-  if (q_batch_stride <= 0 || q_head_stride <= 0 || kv_block_stride <= 0 || kv_token_stride <= 0 ||
-      kv_head_stride <= 0 || out_batch_stride <= 0 || out_head_stride <= 0)
-    return LA_ERR_INVALID_ARGUMENT;
-  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16)) return LA_ERR_ALIGNMENT;
-  if (q_batch_stride % 8 || q_head_stride % 8 || kv_block_stride % 8 || kv_token_stride % 8 || kv_head_stride % 8)
-    return LA_ERR_ALIGNMENT;
-  if (!aligned(out, 8) || out_batch_stride % 4 || out_head_stride % 4) return LA_ERR_ALIGNMENT;
-
+  if (num_groups < 0 || (num_groups > 0 && (!prefix_lens || !cu_prefix_rows))) return LA_ERR_INVALID_ARGUMENT;
+  decode::Call call;
+  int st = decode::prepare_call(q, q_batch_stride, q_head_stride, k_cache, v_cache, kv_block_stride, kv_token_stride,
+                                kv_head_stride, num_blocks, block_size, block_table, bt_seq_stride, max_blocks_per_seq,
+                                cache_seqlens, batch, num_q_heads, num_kv_heads, head_dim, softmax_scale, out,
+                                out_batch_stride, out_head_stride, softmax_lse, dev_error, &call);
+  if (st != LA_OK || batch == 0) return st;
+  if (num_blocks > 0x7ffffffeLL) return LA_ERR_UNSUPPORTED;
   const int device = current_device();
   const int grid = device >= 0 ? num_sms(device) : 0;
   if (grid <= 0) return LA_ERR_CUDA;
-  size_t need = 0;
-  int st = la_paged_decode_shared_prefix_workspace_size(device, batch, num_groups, num_q_heads, num_kv_heads, head_dim,
-                                                        &need);
-  if (st != LA_OK) return st;
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return LA_ERR_WORKSPACE;
-
+  const Workspace w = workspace_of(batch, num_q_heads, num_kv_heads, grid);
+  if (w.rows > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return LA_ERR_WORKSPACE;
   if (num_groups == 0 || batch < 2)  // nothing to share; the workspace is larger than that call's
     return la_paged_decode(q, q_batch_stride, q_head_stride, k_cache, v_cache, kv_block_stride, kv_token_stride,
                            kv_head_stride, num_blocks, block_size, block_table, bt_seq_stride, max_blocks_per_seq,
                            cache_seqlens, batch, num_q_heads, num_kv_heads, head_dim, softmax_scale, out,
                            out_batch_stride, out_head_stride, softmax_lse, workspace, workspace_bytes, dev_error, stream);
 
-  PrefixGroups groups;
+  const int group = num_q_heads / num_kv_heads, per_tile = kRows / group;
+  PrefixGroups& groups = call.p.groups;
   groups.cu = cu_prefix_rows;
   groups.lens = prefix_lens;
   groups.n = num_groups;
   groups.batch = batch;
   groups.block_size = block_size;
-  groups.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
+  groups.bs_shift = call.p.bs_shift;
   groups.cap = static_cast<int64_t>(max_blocks_per_seq) * block_size;
-  if (groups.cap > 0x7fffff00LL) groups.cap = 0x7fffff00LL / block_size * block_size;  // lengths are int32
-  const int per_tile = kRows / group;
-  // the steps of one group, counted in 32 bits
-  const int64_t key_tiles = (groups.cap + kKeys - 1) / kKeys;
-  if (key_tiles * num_kv_heads * (batch / (2 * per_tile) + 1) > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
+  if (groups.cap > 0x7fff0000LL) groups.cap = 0x7fff0000LL / block_size * block_size;  // lengths are int32
+  // steps of all groups and units of 256 rows are counted in 32 bits
+  const int64_t key_tiles = (groups.cap + kKeys - 1) / kKeys, most_groups = num_groups < batch ? num_groups : batch;
+  if (key_tiles * num_kv_heads * (batch / (2 * per_tile) + most_groups) > 0x7fffffffLL ||
+      256 * (groups.cap / call.p.tc + 1) > 0x7fffffffLL)
+    return LA_ERR_UNSUPPORTED;
 
-  const int64_t rows = prefix_rows(batch, num_q_heads, grid), all = rows + own_rows(batch, num_q_heads, grid);
-  float* part_o = static_cast<float*>(workspace);
-  float* part_lse = part_o + all * kD;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Params p;
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_lse = reinterpret_cast<float*>(ws + w.lse);
+  p.items = reinterpret_cast<int4*>(ws + w.items);
+  p.flags = reinterpret_cast<int*>(ws + w.flags);
+  call.p.part_o = p.part_o + w.own0 * kD;
+  call.p.part_lse = p.part_lse + w.own0;
+  call.p.row_parts = reinterpret_cast<int*>(ws + w.parts);
+  p.own = call.p;
+  p.per_tile = per_tile;
+  p.box_keys = kKeys;
+  while (block_size % p.box_keys) p.box_keys >>= 1;
 
+  CUtensorMap tq, tk, tv;
   {
-    CUtensorMap tq, tk, tv;
-    {
-      const uint64_t dims[3] = {128, static_cast<uint64_t>(num_q_heads), static_cast<uint64_t>(batch)};
-      const uint64_t strides[2] = {static_cast<uint64_t>(q_head_stride) * 2, static_cast<uint64_t>(q_batch_stride) * 2};
-      const uint32_t box[3] = {64, static_cast<uint32_t>(group), static_cast<uint32_t>(per_tile)};
-      if ((st = encode_tensor_map_bf16(&tq, q, 3, dims, strides, box, true)) != LA_OK) return st;
-    }
-    int box_keys = kKeys;
-    while (block_size % box_keys) box_keys >>= 1;
-    {
-      const uint64_t dims[4] = {128, static_cast<uint64_t>(block_size), static_cast<uint64_t>(num_kv_heads),
-                                static_cast<uint64_t>(num_blocks)};
-      const uint64_t strides[3] = {static_cast<uint64_t>(kv_token_stride) * 2, static_cast<uint64_t>(kv_head_stride) * 2,
-                                   static_cast<uint64_t>(kv_block_stride) * 2};
-      const uint32_t box[4] = {64, static_cast<uint32_t>(box_keys), 1, 1};
-      if ((st = encode_tensor_map_bf16(&tk, k_cache, 4, dims, strides, box, true)) != LA_OK) return st;
-      if ((st = encode_tensor_map_bf16(&tv, v_cache, 4, dims, strides, box, true)) != LA_OK) return st;
-    }
-    Params p;
-    p.groups = groups;
-    p.table = block_table;
-    p.table_stride = bt_seq_stride;
-    p.max_blocks = max_blocks_per_seq;
-    p.num_blocks = static_cast<int>(num_blocks);
-    p.box_keys = box_keys;
-    p.hkv = num_kv_heads;
-    p.group = group;
-    p.per_tile = per_tile;
-    p.scale_log2 = softmax_scale * 1.4426950408889634f;
-    p.part_o = part_o;
-    p.part_lse = part_lse;
-    p.err = dev_error;
-    st = cuda_status(launch_pdl(prefix_kernel, dim3(grid), dim3(kThreads), kSmemBytes, stream, tq, tk, tv, p));
-    if (st != LA_OK) return st;
+    const uint64_t dims[3] = {128, static_cast<uint64_t>(num_q_heads), static_cast<uint64_t>(batch)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(q_head_stride) * 2, static_cast<uint64_t>(q_batch_stride) * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(group), static_cast<uint32_t>(per_tile)};
+    if ((st = encode_tensor_map_bf16(&tq, q, 3, dims, strides, box, true)) != LA_OK) return st;
   }
-
-  st = decode_own_keys(q, q_batch_stride, q_head_stride, k_cache, v_cache, kv_block_stride, kv_token_stride,
-                       kv_head_stride, num_blocks, block_size, block_table, bt_seq_stride, max_blocks_per_seq,
-                       cache_seqlens, batch, num_q_heads, num_kv_heads, head_dim, softmax_scale, out, out_batch_stride,
-                       out_head_stride, softmax_lse, dev_error, stream,
-                       OwnKeysPass{groups, part_o + rows * kD, part_lse + rows});
+  {
+    const uint64_t dims[4] = {128, static_cast<uint64_t>(block_size), static_cast<uint64_t>(num_kv_heads),
+                              static_cast<uint64_t>(num_blocks)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(kv_token_stride) * 2, static_cast<uint64_t>(kv_head_stride) * 2,
+                                 static_cast<uint64_t>(kv_block_stride) * 2};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(p.box_keys), 1, 1};
+    if ((st = encode_tensor_map_bf16(&tk, k_cache, 4, dims, strides, box, true)) != LA_OK) return st;
+    if ((st = encode_tensor_map_bf16(&tv, v_cache, 4, dims, strides, box, true)) != LA_OK) return st;
+  }
+  size_t smem = 0;
+  const int stages = decode::stages_for(call.p.stage_bytes, kCtrlBytes + call.merge_bytes, &smem);
+  if (stages == 0) return LA_ERR_UNSUPPORTED;
+  if (smem < kSmemBytes) smem = kSmemBytes;
+  st = cuda_status(launch_pdl(stages == 3 ? shared_prefix_kernel<3> : shared_prefix_kernel<2>, dim3(grid),
+                              dim3(kThreads), smem, stream, tq, tk, tv, call.q, call.k, call.v, call.k1, call.v1, p));
   if (st != LA_OK) return st;
 
   CombineParams c;
-  c.groups = groups;
-  c.seqlens = cache_seqlens;
+  c.flags = p.flags;
+  c.row_parts = reinterpret_cast<const int2*>(ws + w.parts);
+  c.items = p.items;
   c.hq = num_q_heads;
   c.hkv = num_kv_heads;
   c.group = group;
-  c.per_tile = per_tile;
   c.grid = grid;
-  c.tc = 16 * (8 / num_kv_heads);
-  c.own0 = static_cast<int>(rows);
-  c.part_o = part_o;
-  c.part_lse = part_lse;
+  c.own0 = static_cast<int>(w.own0);
+  c.rows = static_cast<int>(w.rows);
+  c.part_o = p.part_o;
+  c.part_lse = p.part_lse;
   c.out = static_cast<__nv_bfloat16*>(out);
   c.out_bs = out_batch_stride;
   c.out_hs = out_head_stride;
   c.lse = softmax_lse;
   const int warps = num_q_heads < kCombineWarps ? num_q_heads : kCombineWarps;
-  return cuda_status(launch_pdl(combine_kernel, dim3(batch), dim3(32 * warps), 0, stream, c));
+  return cuda_status(launch_pdl(combine_kernel, dim3(batch, (num_q_heads + warps - 1) / warps), dim3(32 * warps), 0,
+                                stream, c));
 }
