@@ -19,14 +19,13 @@ move_blocks are the device side.
 """
 from __future__ import annotations
 
-import ctypes
 from collections import deque
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from .flash_attn_interface import (_check, _device_index, _ptr, _stream, ensure_init, error_word, paged_kv_write)
+from .flash_attn_interface import _check, _device_index, _raw_stream, ensure_init, error_word, paged_kv_write
 
 
 def blocks_for(n_tokens: int, block_size: int) -> int:
@@ -106,24 +105,25 @@ class BlockAllocator:
 def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple:
     """The pools as la_copy_blocks takes them, from [L, NB, BS, Hkv, D] or one
     layer's [NB, BS, Hkv, D]."""
-    _check(k_pool.dim() in (4, 5) and k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride()
-           and k_pool.dtype == v_pool.dtype and k_pool.device == v_pool.device,
+    shape, stride = k_pool.shape, k_pool.stride()
+    _check(len(shape) in (4, 5) and shape == v_pool.shape and stride == v_pool.stride()
+           and k_pool.dtype is v_pool.dtype and k_pool.device == v_pool.device,
            "k_pool and v_pool must be [num_layers, num_blocks, block_size, num_heads_k, head_dim] (or one layer) of the "
            "same shape, strides and type on one device")
-    _check(k_pool.stride(-1) == 1, "the head_dim axis must be contiguous")
-    layers, layer_stride = (k_pool.shape[0], k_pool.stride(0)) if k_pool.dim() == 5 else (1, 0)
-    nb, bs, heads, dim = k_pool.shape[-4:]
-    return (_ptr(k_pool), _ptr(v_pool), layer_stride, *k_pool.stride()[-4:-1], layers, nb, bs, heads, dim,
+    _check(stride[-1] == 1, "the head_dim axis must be contiguous")
+    layers, layer_stride = (shape[0], stride[0]) if len(shape) == 5 else (1, 0)
+    return (k_pool.data_ptr(), v_pool.data_ptr(), layer_stride, *stride[-4:-1], layers, *shape[-4:],
             k_pool.element_size())
 
 
-def _check_ids(name: str, ids: torch.Tensor, n: int, device: torch.device) -> None:
-    _check(ids.dtype == torch.int32 and ids.shape == (n,) and ids.is_contiguous() and ids.device == device,
+def _ids(name: str, ids: torch.Tensor, n: int, device: torch.device) -> int:
+    _check(ids.dtype is torch.int32 and ids.shape == (n,) and ids.is_contiguous() and ids.device == device,
            f"{name} must be a contiguous int32 [num_pairs] tensor on the pools' device")
+    return ids.data_ptr()
 
 
 def _check_table(block_table: torch.Tensor, device: torch.device) -> None:
-    _check(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.device == device
+    _check(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.device == device
            and block_table.stride(1) == 1 and (block_table.shape[0] < 2 or block_table.stride(0) >= block_table.shape[1]),
            "block_table must be row-contiguous int32 [batch, max_blocks] on the pools' device")
 
@@ -143,14 +143,11 @@ def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Te
     args = _pools(k_pool, v_pool)
     device, n = k_pool.device, src_blocks.numel()
     dev = _device_index(k_pool)
-    _check_ids("src_blocks", src_blocks, n, device)
-    _check_ids("dst_blocks", dst_blocks, n, device)
-    if num_tokens is not None:
-        _check_ids("num_tokens", num_tokens, n, device)
+    src, dst = _ids("src_blocks", src_blocks, n, device), _ids("dst_blocks", dst_blocks, n, device)
+    tokens = _ids("num_tokens", num_tokens, n, device) if num_tokens is not None else None
     with torch.cuda.device(dev):
         ensure_init(dev)
-        _lib.call("la_copy_blocks", *args, _ptr(src_blocks), _ptr(dst_blocks), _ptr(num_tokens), n,
-                  _ptr(error_word(dev)), _stream(device))
+        _lib.call("la_copy_blocks", *args, src, dst, tokens, n, error_word(dev).data_ptr(), _raw_stream(dev))
 
 
 def move_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
@@ -162,15 +159,14 @@ def move_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Te
     args = _pools(k_pool, v_pool)
     device, n = k_pool.device, src_blocks.numel()
     dev = _device_index(k_pool)
-    _check_ids("src_blocks", src_blocks, n, device)
-    _check_ids("dst_blocks", dst_blocks, n, device)
+    src, dst = _ids("src_blocks", src_blocks, n, device), _ids("dst_blocks", dst_blocks, n, device)
     _check_table(block_table, device)
     rows, cols = block_table.shape
     with torch.cuda.device(dev):
         ensure_init(dev)
-        _lib.call("la_move_blocks", *args, _ptr(src_blocks), _ptr(dst_blocks), n,
-                  _ptr(block_table), block_table.stride(0) if rows > 1 else cols, rows, cols,
-                  _ptr(error_word(dev)), _stream(device))
+        _lib.call("la_move_blocks", *args, src, dst, n,
+                  block_table.data_ptr(), block_table.stride(0) if rows > 1 else cols, rows, cols,
+                  error_word(dev).data_ptr(), _raw_stream(dev))
 
 
 def shared_prefix_groups(tables: Sequence[Sequence[int]], lengths: Sequence[int], block_size: int,

@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(32 * kCombinePeerWarps, 1) paged_decode_combin
 }
 
 // ------------------------------------------------------------------ host
-int stages_for(int stage_bytes, size_t ctrl_bytes, size_t* smem) {
+static int stages_for(int stage_bytes, size_t ctrl_bytes, size_t* smem) {
   const size_t limit = 227 * 1024;
   for (int st = 3; st >= 2; --st) {
     const size_t need = 1024 /*align slack*/ + static_cast<size_t>(st) * stage_bytes + ctrl_bytes;

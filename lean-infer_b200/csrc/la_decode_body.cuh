@@ -186,6 +186,21 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
                                         Windows<kPrefix>& w, long long u0, long long n_units, int b0, long long pb0,
                                         int cta, int pid, int nprod, int lane) {
   const int hkv = p.hkv;
+  // kPrefix: a row's own keys are read once, and beside them run CTAs that
+  // read the shared ones, and code, from L2.
+  [[maybe_unused]] const uint64_t once = kPrefix ? l2_evict_first() : 0;
+  auto load4 = [&](void* dst, const CUtensorMap* tm, uint64_t* bar, int c0, int c1, int c2, int c3) {
+    if constexpr (kPrefix)
+      tma_load_4d(dst, tm, bar, c0, c1, c2, c3, once);
+    else
+      tma_load_4d(dst, tm, bar, c0, c1, c2, c3);
+  };
+  auto load5 = [&](void* dst, const CUtensorMap* tm, uint64_t* bar, int c0, int c1, int c2, int c3, int c4) {
+    if constexpr (kPrefix)
+      tma_load_5d(dst, tm, bar, c0, c1, c2, c3, c4, once);
+    else
+      tma_load_5d(dst, tm, bar, c0, c1, c2, c3, c4);
+  };
   // Producer pid issues units k = pid, pid + nprod, ...; every producer
   // walks every unit to follow the sequences. One warp's per-unit path
   // (stage wait, descriptor, four TMA boxes whose issue alone takes ~650
@@ -299,7 +314,7 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
       const int ph0 = __shfl_sync(0xffffffffu, phys, 0);
       const int grp = __shfl_sync(0xffffffffu, off, 0) / kSub;
       if (lane < 4)
-        tma_load_5d(st + tens * kKVBytes + half * kKVHalf, tens ? &tm_v : &tm_k, &full[s], half * 64, 0, 0, grp,
+        load5(st + tens * kKVBytes + half * kKVHalf, tens ? &tm_v : &tm_k, &full[s], half * 64, 0, 0, grp,
                     ph0);
     } else if (p.unit_box) {
       // A sequence's last unit, not full: only the sub-chunks that hold
@@ -313,10 +328,10 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
         const int grp = off / kSub;
         uint8_t* kd = st + lane * kTileBytes;
         uint8_t* vd = st + kKVBytes + lane * kTileBytes;
-        tma_load_5d(kd, &tm_k1, &full[s], 0, 0, 0, grp, phys);
-        tma_load_5d(kd + kKVHalf, &tm_k1, &full[s], 64, 0, 0, grp, phys);
-        tma_load_5d(vd, &tm_v1, &full[s], 0, 0, 0, grp, phys);
-        tma_load_5d(vd + kKVHalf, &tm_v1, &full[s], 64, 0, 0, grp, phys);
+        load5(kd, &tm_k1, &full[s], 0, 0, 0, grp, phys);
+        load5(kd + kKVHalf, &tm_k1, &full[s], 64, 0, 0, grp, phys);
+        load5(vd, &tm_v1, &full[s], 0, 0, 0, grp, phys);
+        load5(vd + kKVHalf, &tm_v1, &full[s], 64, 0, 0, grp, phys);
       }
     } else if (p.big_box) {
       // Sub-chunk j (all kv heads in one box per half, the lane of its head
@@ -327,15 +342,15 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
       const int sof = __shfl_sync(0xffffffffu, off, src);
       const bool sact = __shfl_sync(0xffffffffu, active ? 1 : 0, src) != 0;
       if (jj < p.nsub && sact)
-        tma_load_4d(st + tens * kKVBytes + half * kKVHalf + src * kTileBytes, tens ? &tm_v : &tm_k, &full[s],
+        load4(st + tens * kKVBytes + half * kKVHalf + src * kTileBytes, tens ? &tm_v : &tm_k, &full[s],
                     half * 64, sof, 0, sph);
     } else if (active) {
       uint8_t* kd = st + lane * kTileBytes;
       uint8_t* vd = st + kKVBytes + lane * kTileBytes;
-      tma_load_4d(kd, &tm_k, &full[s], 0, head, off, phys);
-      tma_load_4d(kd + kKVHalf, &tm_k, &full[s], 64, head, off, phys);
-      tma_load_4d(vd, &tm_v, &full[s], 0, head, off, phys);
-      tma_load_4d(vd + kKVHalf, &tm_v, &full[s], 64, head, off, phys);
+      load4(kd, &tm_k, &full[s], 0, head, off, phys);
+      load4(kd + kKVHalf, &tm_k, &full[s], 64, head, off, phys);
+      load4(vd, &tm_v, &full[s], 0, head, off, phys);
+      load4(vd + kKVHalf, &tm_v, &full[s], 64, head, off, phys);
     }
   }
   // On an early exit, let the copies this warp issued land before the CTA
@@ -623,10 +638,6 @@ int prepare_call(const void* q, int64_t q_batch_stride, int64_t q_head_stride, c
                  int max_blocks_per_seq, const int32_t* cache_seqlens, int batch, int num_q_heads, int num_kv_heads,
                  int head_dim, float softmax_scale, void* out, int64_t out_batch_stride, int64_t out_head_stride,
                  float* softmax_lse, int* dev_error, Call* call);
-
-// Pipeline stages (3, 2, or 0 where they do not fit) beside ctrl_bytes of
-// other shared memory, and the shared memory of a CTA.
-int stages_for(int stage_bytes, size_t ctrl_bytes, size_t* smem);
 
 }  // namespace decode
 }  // namespace la

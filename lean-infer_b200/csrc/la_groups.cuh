@@ -24,16 +24,18 @@ struct PrefixGroup {
   int first, rows, keys;
 };
 
-__device__ __forceinline__ PrefixGroup load_group(const PrefixGroups& G, int g) {
+__device__ __forceinline__ PrefixGroup group_from(const PrefixGroups& G, int first, int last, int len) {
   PrefixGroup r;
-  r.first = G.cu[g];
-  const int last = G.cu[g + 1];
-  const long long n = min(static_cast<long long>(max(G.lens[g], 0)), G.cap);
+  r.first = first;
+  const long long n = min(static_cast<long long>(max(len, 0)), G.cap);
   const bool sound = r.first >= 0 && r.first <= last && last <= G.batch;
   r.rows = sound ? last - r.first : 0;
   const int blocks = G.bs_shift >= 0 ? static_cast<int>(n) >> G.bs_shift : static_cast<int>(n) / G.block_size;
   r.keys = r.rows >= 2 ? blocks * G.block_size : 0;
   return r;
+}
+__device__ __forceinline__ PrefixGroup load_group(const PrefixGroups& G, int g) {
+  return group_from(G, G.cu[g], G.cu[g + 1], G.lens[g]);
 }
 
 // From the CTA's table of all groups, where there is room for one.

@@ -32,10 +32,11 @@
 // P equal ranges; an item's part in a range is a segment, which leaves
 // normalised fp32 O rows and base-2 logarithms of its sums.
 //
-// CTA, 16 warps. Shared part: 0-3 and 4-7 softmax of tile 0 and 1 (a thread
-// per row, the S row in registers), 8-11 store the segments' O, 12 issues the
-// products, 13 the TMA loads; tensor memory holds S0 S1 O0 O1, 128 columns
-// each, P over S. Own keys: 0-7 consume, 8 and 9 load.
+// CTA, 12 warps. Shared part: 0-3 and 4-7 softmax of tile 0 and 1 (a thread
+// per row, the S row in registers), which store the segments' O as well, 8
+// issues the products, 9 the TMA loads; tensor memory holds S0 S1 O0 O1, 128
+// columns each, P over S. Own keys: 0-7 consume, 8 and 9 load. 10 makes the
+// plan, 11 sets the barriers up.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -55,50 +56,54 @@ constexpr int kKeys = 128;             // keys per K/V tile
 constexpr int kHalf = 128 * 128;       // 64 dims of 128 rows: 16 KB
 constexpr int kTile = 2 * kHalf;
 constexpr int kStages = 4;             // K/V tiles in flight
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;          // 12 warps: 168 registers for each thread
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;        // O_t at kColO + 128 t; S_t at 128 t
 constexpr uint32_t kIdescQK = idesc_bf16_f32(128, kKeys, false, false);
 constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, false, true);
-// Registers per thread, of the 512 x 128 that the CTA is launched with.
-constexpr int kRegSoftmax = 160, kRegStore = 88, kRegOther = 104;  // shared part: warps 0-7, 8-11, 12-15
-constexpr int kRegConsume = 160, kRegLoad = 104, kRegIdle = 88;    // own keys: the same
-static_assert(256 * kRegSoftmax + 128 * kRegStore + 128 * kRegOther <= kThreads * 128 &&
-                  256 * kRegConsume + 128 * kRegLoad + 128 * kRegIdle <= kThreads * 128,
-              "the register split must fit in the registers the CTA is launched with");
 // Shared memory. Control, both parts' barriers apart: they are initialised
-// before the CTA knows which part it takes. Then the part's data: Q0 Q1, K/V
-// ring, staging of O (4 KB per storing warp), row sums and maxima; or the
-// stages and the merge area of the decode warps.
+// before the CTA knows which part it takes. Then the part's data: Q0 Q1 and the
+// K/V ring; or the stages and the merge area of the decode warps.
 constexpr int kOffOwnBar = 256;
 constexpr int kOffPlan = 384;
+constexpr int kOffStale = 448;
 constexpr int kOffDesc = 512;
 constexpr int kOffZero = 640;
 constexpr int kOffWalk = 768;          // of the softmax warps, kept out of their registers
-constexpr int kWalkBytes = 112;
+constexpr int kWalkBytes = 120;
 constexpr int kOffTable = 2048;
 constexpr int kMaxGroups = 512;        // groups that the table holds; more are read from global memory
 constexpr int kCtrlBytes = 8192;
 constexpr int kOffQ = kCtrlBytes;
 constexpr int kOffKV = kOffQ + 2 * kTile;
-constexpr int kOffStage = kOffKV + kStages * kTile;
-constexpr int kStageBytes = 32 * 128;
-constexpr int kOffStats = kOffStage + 4 * kStageBytes;
-constexpr size_t kSmemBytes = kOffStats + 2 * 2 * kRows * 4 + 1024;  // + alignment to 1024 bytes at run time
+constexpr size_t kSmemBytes = kOffKV + kStages * kTile + 1024;  // + alignment to 1024 bytes at run time
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(kOffWalk + 8 * kWalkBytes <= kOffTable && kOffTable + kMaxGroups * sizeof(PrefixGroup) <= kCtrlBytes,
               "control area");
+// Warps behind the eight of softmax or consumers.
+// Pipeline stages (of 64 KB) of the decode warps. What they keep in flight,
+// 128 KB on each SM, draws all that HBM has; the third stage that fits only
+// makes every load wait longer, and the shared part, whose CTAs keep less in
+// flight, waits with them (128 rows behind 2048 keys: 74 us with three, 61
+// with two).
+constexpr int kOwnStages = 2;
+constexpr int kWarpProduct = 8, kWarpLoad = 9;  // own keys: both load
+constexpr int kWarpPlan = 10, kWarpSetup = 11;
 
-// The time model that divides the SMs (microseconds; measured on a B200 at
-// ~1.9 GHz): a step of the shared part; a unit of 64 KB of a row's own keys
-// on one SM, without and with sub-chunks to merge (nsub > 1); 64 KB at the
-// rate that all SMs together reach.
-constexpr float kStepUs = 2.4f, kUnitUs = 0.8f, kUnitMergedUs = 1.25f, kHbmUs = 0.0109f;
+// The time model that divides the SMs (shared_ctas). Microseconds on a B200 at
+// ~1.9 GHz, fitted to the times of 15 calls with 2 to 146 CTAs for the shared
+// part; of those calls 13 get the division that measured fastest, or one within
+// 2 %, the others one within 11 %. A step with two row tiles (64 KB of K and V), with
+// one (128 KB); a unit (64 KB) of a row's own keys, without and with sub-chunks
+// to merge (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
+constexpr float kPairUs = 3.0f, kSingleUs = 3.6f, kUnitUs = 1.08f, kUnitMergedUs = 1.7f, kHbmUs = 0.0094f,
+                kSegmentUs = 4.0f;
 
 struct Params {
   decode::Params own;  // the rows' own keys; groups, tables, counts and scale of both parts
   int box_keys;        // keys per TMA box, a power of two that divides the block size
   int per_tile;        // sequences per row tile: 128 / group
+  uint32_t tile_magic; // ceil(2^32 / per_tile): x / per_tile is the high word of x * magic for x < 2^25
   float* part_o;       // [rows][D]
   float* part_lse;     // [rows], base 2
   int4* items;         // [batch][hkv]: first partial row of the row's first head, distance of the second
@@ -113,21 +118,23 @@ struct Shape {
   int tiles;    // key tiles
   int pairs;    // of row tiles, the single one included
   int single;   // 1: the last has one tile
+  int half;     // steps of that one
   int per_head; // steps of one kv head
 };
 
-__device__ __forceinline__ Shape shape_of(const PrefixGroup& g, int per_tile) {
+__device__ __forceinline__ Shape shape_of(const Params& p, const PrefixGroup& g) {
   Shape s;
-  const int row_tiles = (g.rows + per_tile - 1) / per_tile;
+  const int row_tiles = static_cast<int>(__umulhi(g.rows + p.per_tile - 1, p.tile_magic));
   s.tiles = (g.keys + kKeys - 1) / kKeys;
   s.pairs = (row_tiles + 1) >> 1;
   s.single = row_tiles & 1;
-  s.per_head = (s.pairs - s.single) * s.tiles + (s.single ? (s.tiles + 1) >> 1 : 0);
+  s.half = s.single ? (s.tiles + 1) >> 1 : 0;
+  s.per_head = (s.pairs - s.single) * s.tiles + s.half;
   return s;
 }
 
 __device__ __forceinline__ int steps_of(const Params& p, const PrefixGroup& g) {
-  return g.keys > 0 ? p.own.hkv * shape_of(g, p.per_tile).per_head : 0;
+  return g.keys > 0 ? p.own.hkv * shape_of(p, g).per_head : 0;
 }
 
 // First partial row of item (g, h, r) in CTA c. An item's segments take up to
@@ -138,20 +145,16 @@ __device__ __forceinline__ int part_row(const Params& p, const PrefixGroup& g, i
   return 2 * p.own.group * (p.own.hkv * g.first + h * g.rows + r * 2 * p.per_tile) + 2 * kRows * c;
 }
 
-// What the CTA does: its range of steps (P > blockIdx.x) or of units, and
-// where that begins.
+// What the CTA does: its range of steps or of units, and where that begins.
 struct Plan {
   long long u0, u1;
   long long before;  // steps before group `at`, or units before row `at`
   int at;
-  int P;             // CTAs of the shared part
+  int shared;        // takes part in the shared part
+  int c;             // its number in its part
 };
 
-__device__ __forceinline__ int warp_sum(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 __device__ __forceinline__ int warp_scan(int v, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -162,7 +165,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
 }
 
 // Lengths of rows base + 8 lane + i (0 past the batch), 16 bytes at a time
-// where they can be.
+// where they can be; through L2 only, since the kernel in front may still
+// write them (no stale line stays in L1).
 __device__ __forceinline__ void load_lens8(const Params& p, int lane, int base, int (&raw)[8]) {
   const int* s = p.own.seqlens;
   const int b0 = base + 8 * lane;
@@ -171,82 +175,167 @@ __device__ __forceinline__ void load_lens8(const Params& p, int lane, int base, 
   for (int v = 0; v < 2; ++v) {
     const int b = b0 + 4 * v;
     if (vec && b + 3 < p.own.batch) {
-      const int4 x = *reinterpret_cast<const int4*>(s + b);
+      const int4 x = __ldcg(reinterpret_cast<const int4*>(s + b));
       raw[4 * v] = x.x;
       raw[4 * v + 1] = x.y;
       raw[4 * v + 2] = x.z;
       raw[4 * v + 3] = x.w;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) raw[4 * v + e] = b + e < p.own.batch ? s[b + e] : 0;
+      for (int e = 0; e < 4; ++e) raw[4 * v + e] = b + e < p.own.batch ? __ldcg(s + b + e) : 0;
     }
   }
 }
 
-// Units of those rows (kept in raw), and their sum.
-__device__ __forceinline__ int units8(const Params& p, const PrefixGroup* tab, int lane, int base, int (&raw)[8]) {
-  int sum = 0;
-#pragma unroll 1
-  for (int i = 0; i < 8; ++i) {
-    int c = raw[0];
-    c = c < 0 ? 0 : c > p.own.groups.cap ? static_cast<int>(p.own.groups.cap) : c;
-    if (c > 0) c -= prefix_keys(p.own.groups, tab, base + 8 * lane + i, c);
-    const int n = decode::units_p(p.own, c);
-    sum += n;
+// What a plan for up to 256 rows and 32 groups was made from, one warp.
+struct Seen {
+  int raw[8];
+  int lo, hi, len;
+};
+__device__ __forceinline__ Seen read_inputs(const Params& p, int lane) {
+  Seen r;
+  load_lens8(p, lane, 0, r.raw);
+  const bool in = lane < p.own.groups.n;
+  r.lo = in ? __ldcg(p.own.groups.cu + lane) : 0;
+  r.hi = in ? __ldcg(p.own.groups.cu + lane + 1) : 0;
+  r.len = in ? __ldcg(p.own.groups.lens + lane) : 0;
+  return r;
+}
+
+// Units of those rows (kept in raw), and their sum. The first block's look-up
+// of groups runs over the registers of the lanes that hold them (grp: lane g's
+// group, the first of at most 32), the others search the table.
+__device__ __forceinline__ int units8(const Params& p, const PrefixGroup* tab, const PrefixGroup& grp, bool in_regs,
+                                      int lane, int base, int (&raw)[8]) {
+  const int cap = static_cast<int>(p.own.groups.cap);
 #pragma unroll
-    for (int e = 0; e < 7; ++e) raw[e] = raw[e + 1];  // the loop is kept short: its code is cold
-    raw[7] = n;
+  for (int i = 0; i < 8; ++i) raw[i] = min(max(raw[i], 0), cap);
+  if (in_regs) {
+    int own[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own[i] = raw[i];
+    for (int g = 0; g < p.own.groups.n; ++g) {
+      const int d = base + 8 * lane - __shfl_sync(0xffffffffu, grp.first, g);
+      const unsigned rows = __shfl_sync(0xffffffffu, grp.rows, g);
+      const int keys = __shfl_sync(0xffffffffu, grp.keys, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (static_cast<unsigned>(d + i) < rows && raw[i] >= keys) own[i] = raw[i] - keys;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = own[i];
+  } else {
+    for (int i = 0; i < 8; ++i) {
+      const int c = raw[0];
+#pragma unroll
+      for (int e = 0; e < 7; ++e) raw[e] = raw[e + 1];
+      raw[7] = c > 0 ? c - prefix_keys(p.own.groups, tab, base + 8 * lane + i, c) : 0;
+    }
+  }
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    raw[i] = decode::units_p(p.own, raw[i]);
+    sum += raw[i];
   }
   return sum;
 }
 
+// First of T steps or units of CTA c of G; T counts that fit are divided in 32
+// bits, in a fraction of the time.
+__device__ __forceinline__ long long part_start(int c, long long T, int G) {
+  if (T < (1 << 22)) return static_cast<unsigned>(c) * static_cast<unsigned>(T) / static_cast<unsigned>(G);
+  return c * T / G;
+}
+
+// CTAs of the shared part, an even number, from its steps, the rows' units and
+// the items: the one of least time by a model, 64 numbers of CTAs tried at
+// once. Both parts take the time of their work over their CTAs; where all CTAs
+// together would load more than HBM gives, by a factor f, the steps with two
+// row tiles, whose loads are needed soonest, take f^3 as long, the others,
+// whose loads are twice as many, f^0.5. A CTA whose range is not within one
+// item has two segments to store.
+__device__ __forceinline__ int shared_ctas(const Params& p, long long pair_steps, long long single_steps,
+                                           long long units, int items, int grid, int lane) {
+  const float a = static_cast<float>(pair_steps), b = static_cast<float>(single_steps), u = static_cast<float>(units);
+  const float work = a * kPairUs + b * kSingleUs, unit = p.own.nsub > 1 ? kUnitMergedUs : kUnitUs;
+  const float loads = __fdividef(a + 2.f * b, work);  // 64 KB per us and CTA
+  float best = 3e38f;
+  int at = 2;
+  for (int P = 2 + 2 * lane; P <= grid; P += 64) {
+    const float cs = fminf(static_cast<float>(P), a + b), co = fminf(static_cast<float>(grid - P), u);
+    const float f = fmaxf(1.f, (cs * loads + __fdividef(co, unit)) * kHbmUs);
+    const float shared = __fdividef(a * kPairUs * f * f * f + b * kSingleUs * sqrtf(f), cs) +
+                         (P % items ? kSegmentUs : 0.f);
+    const float own = u > 0.f ? (co > 0.f ? __fdividef(u * unit, co) : 1e38f) : 0.f;
+    const float t = fmaxf(shared, own);
+    if (t < best) {
+      best = t;
+      at = P;
+    }
+  }
+  // positive floats compare as their bits do
+  const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(best));
+  return static_cast<int>(__reduce_min_sync(0xffffffffu, __float_as_uint(best) == least ? at : 0x7fffffffu));
+}
+
 // One warp's work. tab: the table to fill, or null where the groups exceed it.
-__device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, int lane) {
+// in: the first 256 rows and 32 groups.
+__device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, const Seen& in, int lane) {
   const PrefixGroups& G = p.own.groups;
   int raw[8];
-  load_lens8(p, lane, 0, raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) raw[i] = in.raw[i];
   // the shared part: steps, and key tiles that are read
-  long long S = 0, tiles = 0;
+  long long S = 0, single = 0;
+  int items = 0;
+  PrefixGroup grp{0, 0, 0};
   for (int b = 0; b < G.n; b += 32) {
     const int g = b + lane;
-    int s = 0, t = 0;
+    int s = 0, s1 = 0, t = 0;
     if (g < G.n) {
-      const PrefixGroup r = load_group(G, g);
+      const PrefixGroup r = b == 0 ? group_from(G, in.lo, in.hi, in.len) : load_group(G, g);
+      if (b == 0) grp = r;
       if (tab) tab[g] = r;
-      if (blockIdx.x == 0 && p.own.err && (r.first < 0 || G.cu[g + 1] < r.first || G.cu[g + 1] > G.batch))
-        atomicCAS(p.own.err, 0, LA_DEVERR_PREFIX);
-      s = steps_of(p, r);
-      t = p.own.hkv * ((r.keys + kKeys - 1) / kKeys);
+      if (r.keys > 0) {
+        const Shape h = shape_of(p, r);
+        s = p.own.hkv * h.per_head;
+        s1 = p.own.hkv * h.half;
+        t = p.own.hkv * h.pairs;
+      }
     }
     S += warp_sum(s);
-    tiles += warp_sum(t);
+    single += warp_sum(s1);
+    items += warp_sum(t);
   }
   __syncwarp();
   // the rows' own keys: units
-  long long U = 0;
-  const int first = units8(p, tab, lane, 0, raw);
-  U = warp_sum(first);
+  const bool in_regs = G.n <= 32;
+  const int first = units8(p, tab, grp, in_regs, lane, 0, raw);
+  long long U = warp_sum(first);
   for (int base = 256; base < G.batch; base += 256) {
     int x[8];
     load_lens8(p, lane, base, x);
-    U += warp_sum(units8(p, tab, lane, base, x));
+    U += warp_sum(units8(p, tab, grp, in_regs, lane, base, x));
   }
   const int grid = static_cast<int>(gridDim.x);
-  const float a = static_cast<float>(S) * kStepUs;
-  const float own = static_cast<float>(U) * (p.own.nsub > 1 ? kUnitMergedUs : kUnitUs);
-  const float T = fmaxf(static_cast<float>(U + tiles) * kHbmUs, (a + own) / static_cast<float>(grid));
+  const int Q = S > 0 ? (grid - shared_ctas(p, S - single, single, U, items, grid, lane)) & ~1 : grid;
+  // Neighbouring CTAs mostly land on the two SMs of a TPC, next pairs on the
+  // same GPC. A pair has the same part (two that stream load 114 GB/s together,
+  // one beside a tensor core CTA ~48 GB/s while that one takes 1.3 times as
+  // long), and the pairs that stream are spread evenly among the others.
+  const int pairs = grid >> 1, pair = static_cast<int>(blockIdx.x >> 1), before = pair * (Q >> 1) / pairs;
   Plan r;
-  r.P = 0;
-  if (S > 0) {
-    const int most = grid - (U > 0 ? 1 : 0);
-    r.P = max(1, min(static_cast<int>(ceilf(a / T)), static_cast<int>(S < most ? S : most)));
-  }
+  r.shared = S > 0 && (pair >= pairs || (pair + 1) * (Q >> 1) / pairs == before);
+  r.c = r.shared ? static_cast<int>(blockIdx.x) - 2 * min(before, Q >> 1) : 2 * before + static_cast<int>(blockIdx.x & 1);
   r.u0 = r.u1 = r.before = 0;
   r.at = 0;
-  const int c = static_cast<int>(blockIdx.x);
-  if (c < r.P) {
-    r.u0 = decode::cta_start(c, S, r.P);
-    r.u1 = decode::cta_start(c + 1, S, r.P);
+  if (r.shared) {
+    const int n = static_cast<int>(S < grid - Q ? S : grid - Q);
+    if (r.c < n) {
+      r.u0 = part_start(r.c, S, n);
+      r.u1 = part_start(r.c + 1, S, n);
+    }
     long long acc = 0;
     for (int b = 0; b < G.n; b += 32) {  // the group of the first step
       const int s = b + lane < G.n ? steps_of(p, prefix_group(G, tab, b + lane)) : 0;
@@ -262,16 +351,16 @@ __device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, int
     }
   } else {
     // no more CTAs than units, so that a row's parts are those of consecutive ones
-    const long long Q = U < grid - r.P ? U : grid - r.P;
-    if (c - r.P < Q) {
-      r.u0 = decode::cta_start(c - r.P, U, Q);
-      r.u1 = decode::cta_start(c - r.P + 1, U, Q);
+    const int n = static_cast<int>(U < Q ? U : Q);
+    if (r.c < n) {
+      r.u0 = part_start(r.c, U, n);
+      r.u1 = part_start(r.c + 1, U, n);
       long long acc = 0;
       for (int base = 0; base < G.batch; base += 256) {  // the row of the first unit
         int sum = first;
         if (base > 0) {
           load_lens8(p, lane, base, raw);
-          sum = units8(p, tab, lane, base, raw);
+          sum = units8(p, tab, grp, in_regs, lane, base, raw);
         }
         const int incl = warp_scan(sum, lane);
         const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
@@ -304,6 +393,7 @@ __device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, int
 // Segments of the CTA's range, one after another (the same in every thread).
 struct Walk {
   int left;  // steps of the range not yet taken
+  int c;     // the CTA's number in the shared part
   int g, h, r, s;
   PrefixGroup grp;
   Shape shp;
@@ -318,16 +408,18 @@ struct Segment {
   int keys;         // of the group
   int row0;         // first partial row
   int begin, end;   // of the item
+  int c;            // the CTA's number in the shared part
 };
 
 __device__ __forceinline__ void walk_group(const Params& p, const PrefixGroup* tab, Walk& w, int g) {
   w.g = g;
   w.grp = prefix_group(p.own.groups, tab, g);
-  w.shp = shape_of(w.grp, p.per_tile);
+  w.shp = shape_of(p, w.grp);
 }
 
 __device__ __forceinline__ void walk_start(const Params& p, const PrefixGroup* tab, const Plan& R, Walk& w) {
   w.left = static_cast<int>(R.u1 - R.u0);
+  w.c = R.c;
   if (w.left <= 0) return;
   walk_group(p, tab, w, R.at);
   const int x = static_cast<int>(R.u0 - R.before);
@@ -351,7 +443,8 @@ __device__ __forceinline__ bool walk_next(const Params& p, const PrefixGroup* ta
   e.tile0 = one ? 2 * w.s : w.s;
   e.tiles = one ? min(2 * n, w.shp.tiles - e.tile0) : n;
   e.keys = w.grp.keys;
-  e.row0 = part_row(p, w.grp, w.h, w.r, blockIdx.x);
+  e.c = w.c;
+  e.row0 = part_row(p, w.grp, w.h, w.r, w.c);
   e.begin = w.s == 0;
   e.end = w.s + n == steps;
   w.left -= n;
@@ -391,15 +484,6 @@ __device__ __forceinline__ uint64_t desc_kmajor(const uint8_t* tile) {
 }
 __device__ __forceinline__ uint64_t desc_v(const uint8_t* tile) { return smem_desc_sw128(smem_u32(tile), kHalf, 1024); }
 
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // The barriers of the shared part.
 struct Bars {
   uint64_t* b;
@@ -410,25 +494,30 @@ struct Bars {
   __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2] S_t written
   __device__ __forceinline__ uint64_t* s_free() const { return b + 12; }   // [2] P_t V done
   __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2] P_t written (128 arrivals)
-  __device__ __forceinline__ uint64_t* o_empty() const { return b + 16; }  // [2] O_t read by the storing warps (128)
-  __device__ __forceinline__ uint64_t* st_full() const { return b + 18; }  // [2] row sums and maxima of tile t written (128)
-  __device__ __forceinline__ uint64_t* st_empty() const { return b + 20; } // [2] ... and read (128)
+  __device__ __forceinline__ uint64_t* o_empty() const { return b + 16; }  // [2] O_t stored (128)
+  __device__ __forceinline__ uint64_t* planned() const { return b + 18; }  // the plan is in shared memory
+  __device__ __forceinline__ uint64_t* checked() const { return b + 19; }  // it was checked after the wait
+  __device__ __forceinline__ uint64_t* done() const { return b + 20; }     // a softmax warp is through (8)
 };
 
 __device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.own.err, LA_DEVERR_WAIT_TIMEOUT));
 }
 
-// Softmax of tile t, four warps, a thread per row.
+// Softmax of tile t and the segments' results, four warps, a thread per row.
+// begin() brings the plan: called once, after a first round over whatever the
+// S columns hold, which writes nothing. That round fetches the code while the
+// lengths, and then the first tiles, are on their way; fetched line by line as
+// the first tile ran, beside CTAs that fill HBM, it took up to 16 us.
+template <typename Begin>
 __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
-                                             Bars bars, uint32_t tmem, int t, int warp, int lane) {
+                                             Bars bars, uint32_t tmem, int t, int warp, int lane, Begin begin) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* s_full = bars.s_full();
+  uint64_t* s_free = bars.s_free();
   uint64_t* p_full = bars.p_full();
-  uint64_t* st_full = bars.st_full();
-  uint64_t* st_empty = bars.st_empty();
+  uint64_t* o_empty = bars.o_empty();
   const float NEG_INF = -__int_as_float(0x7f800000);
-  float* stats = reinterpret_cast<float*>(smem + kOffStats);  // [tile][l | m][128]
   const int quarter = warp & 3;
   const int row = quarter * 32 + lane;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -436,12 +525,6 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
   const float sl2 = p.own.scale_log2;
   Walk& w = *reinterpret_cast<Walk*>(smem + kOffWalk + warp * kWalkBytes);
   Segment& e = *reinterpret_cast<Segment*>(smem + kOffWalk + warp * kWalkBytes + 64);
-  {
-    Walk x;
-    walk_start(p, tab, plan, x);
-    if (lane == 0) w = x;
-    __syncwarp();
-  }
   auto next = [&]() -> bool {
     Walk x = w;
     Segment y{};
@@ -454,15 +537,26 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
     __syncwarp();
     return more;
   };
-  uint32_t seen = 0, nst = 0;  // S tiles, segments with statistics
-  bool ok = true;
-  while (ok && next()) {
+  uint32_t seen = 0;  // S tiles
+  bool ok = true, dry = true;
+  if (lane == 0) {  // the first round's segment: a full key tile, rows of which none is stored
+    e = Segment{};
+    e.two = e.tiles = 1;
+    e.keys = kKeys;
+  }
+  __syncwarp();
+  while (dry || (ok && next())) {
     const int n = tiles_of(e, t);
-    if (n == 0) continue;
-    const bool active = quarter * 32 < rows_of(p, e, t);  // rows of this warp
+    const int rows = dry ? 0 : rows_of(p, e, t);
+    const int row0 = e.row0 + t * rows_of(p, e, 0);
+    if (n == 0) {  // a single key tile: none for the second accumulator
+      if (row < rows) p.part_lse[row0 + row] = NEG_INF;
+      continue;
+    }
+    const bool active = dry || quarter * 32 < rows;  // rows of this warp
     float m = NEG_INF, l = 0.f;
     for (int j = 0; j < n; ++j, ++seen) {
-      if (!(ok = wait_all(&s_full[t], seen & 1))) break;
+      if (!dry && !(ok = wait_all(&s_full[t], seen & 1))) break;
       if (!active) {
         mbar_arrive(&p_full[t]);
         continue;
@@ -519,7 +613,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
           acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
           pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
         }
-        tmem_st32(taddr + colS + c2 * 32, pk);
+        if (!dry) tmem_st32(taddr + colS + c2 * 32, pk);
       }
       float ps[8];
 #pragma unroll
@@ -539,105 +633,93 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
         }
       }
       m = m_new;
+      if (dry) break;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[t]);
     }
     if (!ok) break;
-    if (!(ok = wait_all(&st_empty[t], (nst & 1) ^ 1u))) break;
-    stats[(t * 2 + 0) * kRows + row] = l;
-    stats[(t * 2 + 1) * kRows + row] = m;
-    mbar_arrive(&st_full[t]);
-    ++nst;
-  }
-}
-
-// The segments' results, four warps.
-__device__ __forceinline__ void store_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
-                                           Bars bars, uint32_t tmem, int warp, int lane) {
-  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
-  uint64_t* s_free = bars.s_free();
-  uint64_t* o_empty = bars.o_empty();
-  uint64_t* st_full = bars.st_full();
-  uint64_t* st_empty = bars.st_empty();
-  const float NEG_INF = -__int_as_float(0x7f800000);
-  const float* stats = reinterpret_cast<const float*>(smem + kOffStats);
-  const int quarter = warp & 3;
-  const int row = quarter * 32 + lane;
-  const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  uint8_t* stage = smem + kOffStage + quarter * kStageBytes;
-  Walk w;
-  Segment e{};
-  walk_start(p, tab, plan, w);
-  uint32_t done[2] = {0, 0};  // products P_t V, this segment's included
-  uint32_t segs[2] = {0, 0};
-  bool ok = true;
-  while (ok && walk_next(p, tab, w, e)) {
-    for (int t = 0; t < 2 && ok; ++t) {
-      const int rows = rows_of(p, e, t);
-      const int n = tiles_of(e, t);
-      const int row0 = e.row0 + t * rows_of(p, e, 0);
-      if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
-        int4* it = p.items + static_cast<long long>(e.first + t * p.per_tile + row / p.own.group) * p.own.hkv + e.h;
-        if (e.begin) {
-          it->x = row0 + row;
-          it->y = e.two ? 0 : rows;
-          it->z = static_cast<int>(blockIdx.x);
-        }
-        if (e.end) it->w = static_cast<int>(blockIdx.x);
+    if (!dry && !(ok = wait_all(&s_free[t], (seen - 1) & 1))) break;  // the last product
+    tc_fence_after();
+    // What the combine pass has to know of the item: where its parts are.
+    if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
+      int4* it = p.items + static_cast<long long>(e.first + t * p.per_tile + row / p.own.group) * p.own.hkv + e.h;
+      if (e.begin) {
+        it->x = row0 + row;
+        it->y = e.two ? 0 : rows;
+        it->z = e.c;
       }
-      if (n == 0) {  // a single key tile: none for the second accumulator
-        if (row < rows) p.part_lse[row0 + row] = NEG_INF;
-        continue;
-      }
-      done[t] += n;
-      if (!(ok = wait_all(&st_full[t], segs[t] & 1))) break;
-      const float l = stats[(t * 2 + 0) * kRows + row];
-      const float m = stats[(t * 2 + 1) * kRows + row];
-      mbar_arrive(&st_empty[t]);
-      if (!(ok = wait_all(&s_free[t], (done[t] - 1) & 1))) break;  // the last product
-      tc_fence_after();
-      ++segs[t];
-      if (quarter * 32 >= rows) {
-        mbar_arrive(&o_empty[t]);
-        continue;
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      if (row < rows) p.part_lse[row0 + row] = l == 0.f ? NEG_INF : m + __log2f(l);
-      // 32 columns at a time through the staging buffer (16-byte chunks
-      // XORed by row), so that a store instruction writes 4 rows of 128 bytes.
+      if (e.end) it->w = e.c;
+    }
+    if (row < rows) p.part_lse[row0 + row] = l == 0.f ? NEG_INF : m + __log2f(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // Each thread stores its row, 32 bytes (a sector) at a time.
+    float* dst = p.part_o + static_cast<long long>(row0 + row) * kD;
+    if (active) {
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float o[32];
-        tmem_ld32(taddr + kColO + t * 128 + c * 32, o);
+        tmem_ld32(taddr + colO + c * 32, o);
         tc_wait_ld();
-        if (c == 3) {
-          tc_fence_before();
-          mbar_arrive(&o_empty[t]);
-        }
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          *reinterpret_cast<float4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-              make_float4(o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv);
-        __syncwarp();
+        for (int x = 0; x < 32; ++x) o[x] *= inv;
+        if (row < rows) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = x * 4 + (lane >> 3), ch = lane & 7;
-          const float4 u = *reinterpret_cast<const float4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
-          if (quarter * 32 + r < rows)
-            *reinterpret_cast<float4*>(p.part_o + static_cast<long long>(row0 + quarter * 32 + r) * kD + c * 32 +
-                                       ch * 4) = u;
+          for (int x = 0; x < 4; ++x) store_f32x8(dst + c * 32 + x * 8, o + x * 8);
         }
-        __syncwarp();
       }
     }
+    if (dry) {
+      dry = false;
+      if (!begin()) return;
+      Walk x;
+      walk_start(p, tab, plan, x);
+      if (lane == 0) w = x;
+      __syncwarp();
+      continue;
+    }
+    tc_fence_before();
+    mbar_arrive(&o_empty[t]);
   }
 }
 
-// TMA loads of the shared part, one warp.
+// The page ids of a segment's boxes, one box (64 dims of box_keys keys of one
+// page) per lane: read 32 boxes at a time, the next 32 in advance.
+struct Pages {
+  const int* ids_of_row;
+  int boxes, per_page;  // boxes of a tile, of a page
+  int win, ids, next;
+  __device__ __forceinline__ int read(const Params& p, const Segment& e, int w0, int lane) const {
+    const int x = w0 * 32 + lane;
+    return x * p.box_keys < e.keys ? __ldg(ids_of_row + x / per_page) : -1;
+  }
+  __device__ __forceinline__ void start(const Params& p, const Segment& e, int lane) {
+    boxes = kKeys / p.box_keys;
+    per_page = p.own.block_size / p.box_keys;
+    ids_of_row = p.own.block_table + static_cast<long long>(e.table_row) * p.own.bt_stride;
+    win = e.tile0 * boxes >> 5;
+    ids = read(p, e, win, lane);
+    next = read(p, e, win + 1, lane);
+  }
+  // The page of this lane's box (lane / 2) of a tile; tiles in ascending order.
+  __device__ __forceinline__ int of(const Params& p, const Segment& e, int tile, int lane) {
+    const int x = tile * boxes;
+    if (x >> 5 != win) {
+      win = x >> 5;
+      ids = next;
+      next = read(p, e, win + 1, lane);
+    }
+    return __shfl_sync(0xffffffffu, ids, (x & 31) + min(lane >> 1, boxes - 1));
+  }
+};
+
+// TMA loads of the shared part, one warp, from segment e on (work: there is
+// one, its page ids in `pages`). Per segment Q, then the tiles in the order the
+// products use them: `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1
+// for two row tiles, 2 for the two accumulators of one.
 __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                                          const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
-                                          Bars bars, int lane) {
+                                          const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars, Walk& w,
+                                          Segment& e, bool work, Pages& pages, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* q_full = bars.q_full();
   uint64_t* q_empty = bars.q_empty();
@@ -645,84 +727,57 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
   uint64_t* kv_empty = bars.kv_empty();
   uint8_t* sQ = smem + kOffQ;
   uint8_t* sKV = smem + kOffKV;
-  Walk w;
-  Segment e{};
-  // Per segment Q, then the tiles in the order the products use them:
-  // `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1 for two row
-  // tiles, 2 for the two accumulators of one.
-  walk_start(p, tab, plan, w);
   int kq = 0;
   uint32_t pos = 0;  // tiles loaded
   bool ok = true;
-  // A box per lane: 64 dims of box_keys keys of one page. The page ids of the
-  // segment's boxes are read 32 at a time, the next 32 in advance; V uses the
-  // ids of its K tile, one or two tiles ago.
-  const int boxes = kKeys / p.box_keys, half = lane & 1, box = lane >> 1;
-  const int per_page = p.own.block_size / p.box_keys;  // boxes of a page
-  const int* row_ids = nullptr;
-  int win = -1, ids = 0, next_ids = 0;
-  int k_id = 0, v_id = 0;  // the last K tile's, and the one that the next V tile takes
-  auto read_ids = [&](const Segment& e, int w0) -> int {
-    const int x = w0 * 32 + lane;
-    return x * p.box_keys < e.keys ? __ldg(row_ids + x / per_page) : -1;
-  };
-  auto start = [&](const Segment& e) {
-    row_ids = p.own.block_table + static_cast<long long>(e.table_row) * p.own.bt_stride;
-    win = e.tile0 * boxes >> 5;
-    ids = read_ids(e, win);
-    next_ids = read_ids(e, win + 1);
-  };
-  auto load = [&](const CUtensorMap* tm, const Segment& e, int tile, int id) -> bool {
+  const int half = lane & 1, box = lane >> 1;
+  int k_id = 0, v_id = 0;  // pages of the last K tile, and of the one before
+  auto load = [&](const CUtensorMap* tm, int tile, int id) -> bool {
     const int st = pos % kStages;
     if (!wait_all(&kv_empty[st], ((pos / kStages) & 1) ^ 1u)) return false;
     uint8_t* dst = sKV + st * kTile;
     if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTile);
     __syncwarp();
-    if (box < boxes) {
+    if (box < pages.boxes) {
       // keys behind the prefix, and pages outside the pool, come from block
       // num_blocks, outside the tensor map: zeros
-      const int x = tile * boxes + box;
+      const int x = tile * pages.boxes + box;
       const bool in = x * p.box_keys < e.keys;
       const bool sound = id >= 0 && id < p.own.num_blocks;
       if (in && !sound && p.own.err) atomicCAS(p.own.err, 0, LA_DEVERR_BLOCK_ID);
       const int blk = in && sound ? id : static_cast<int>(p.own.num_blocks);
       tma_load_4d(dst + half * kHalf + box * p.box_keys * 128, tm, &kv_full[st], half * 64,
-                  x % per_page * p.box_keys, e.h, blk);
+                  x % pages.per_page * p.box_keys, e.h, blk);
     }
     __syncwarp();
     ++pos;
     return true;
   };
-  auto load_k = [&](const Segment& e, int tile) -> bool {
-    const int x = tile * boxes;
-    if (x >> 5 != win) {
-      win = x >> 5;
-      ids = next_ids;
-      next_ids = read_ids(e, win + 1);
-    }
-    v_id = k_id;
-    k_id = __shfl_sync(0xffffffffu, ids, (x & 31) + min(box, boxes - 1));
-    return load(&tm_k, e, tile, k_id);
-  };
-  while (ok && walk_next(p, tab, w, e)) {
-    start(e);
+  while (work) {
     if (!(ok = wait_all(q_empty, (kq & 1) ^ 1u))) break;
     if (lane == 0) {
-      const uint32_t half = 128u * p.own.group * p.per_tile;
-      mbar_arrive_expect_tx(q_full, (1 + e.two) * 2 * half);
+      const uint32_t bytes = 128u * p.own.group * p.per_tile;
+      mbar_arrive_expect_tx(q_full, (1 + e.two) * 2 * bytes);
       for (int t = 0; t < 1 + e.two; ++t)
         for (int x = 0; x < 2; ++x)
           tma_load_3d(sQ + t * kTile + x * kHalf, &tm_q, q_full, x * 64, e.h * p.own.group, e.first + t * p.per_tile);
     }
     __syncwarp();
     ++kq;
+    // K(i) and V(i - lead), K first
     const int lead = 2 - e.two;
-    for (int i = 0; ok && i < min(lead, e.tiles); ++i) ok = load_k(e, e.tile0 + i);
-    for (int i = 0; ok && i < e.tiles; ++i) {
-      // the K tile before last where one more is already loaded
-      ok = load(&tm_v, e, e.tile0 + i, lead == 2 && i + 1 < e.tiles ? v_id : k_id);
-      if (ok && i + lead < e.tiles) ok = load_k(e, e.tile0 + i + lead);
+    for (int i = 0; ok && i < e.tiles + lead; ++i) {
+      const int id = v_id;
+      v_id = k_id;
+      if (i >= lead) ok = load(&tm_v, e.tile0 + i - lead, lead == 2 ? id : v_id);
+      if (i < e.tiles) {
+        k_id = pages.of(p, e, e.tile0 + i, lane);
+        ok = ok && load(&tm_k, e.tile0 + i, k_id);
+      }
     }
+    if (!ok) break;
+    work = walk_next(p, tab, w, e);
+    if (work) pages.start(p, e, lane);
   }
   if (!ok && lane == 0) {  // early exit: let the copies already issued land (bounded)
     for (uint32_t u = (pos > kStages ? pos - kStages : 0); u < pos; ++u)
@@ -733,8 +788,8 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
 }
 
 // Products of the shared part, one warp; lane 0 issues.
-__device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
-                                             Bars bars, uint32_t tmem, int lane) {
+__device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars,
+                                             uint32_t tmem, Walk& w, Segment& e, bool work, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* q_full = bars.q_full();
   uint64_t* q_empty = bars.q_empty();
@@ -746,11 +801,8 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
   uint64_t* o_empty = bars.o_empty();
   uint8_t* sQ = smem + kOffQ;
   uint8_t* sKV = smem + kOffKV;
-  Walk w;
-  Segment e{};
   // S_t over P_t is issued right behind the product that reads P_t: the
   // tensor core executes one thread's products in order.
-  walk_start(p, tab, plan, w);
   int kq = 0;
   uint32_t pos = 0;
   uint32_t cp[2] = {0, 0}, segs[2] = {0, 0};
@@ -791,7 +843,7 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
     if (lane == 0) umma_commit(bar);
     __syncwarp();
   };
-  while (ok && walk_next(p, tab, w, e)) {
+  while (work) {
     if (!(ok = wait_all(q_full, kq & 1))) break;
     ++kq;
     const int n = e.tiles, lead = 2 - e.two;
@@ -828,12 +880,19 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
       if (more) release(&kv_empty[kp % kStages]);
       if (more && i + 1 + lead == n) release(q_empty);  // the segment's last S
     }
+    if (!ok) break;
+    work = walk_next(p, tab, w, e);
   }
   __syncwarp();
 }
 
-// What the combine pass has to read of each row, one warp.
+// What the combine pass has to read of each row, and whether the groups are
+// sound; one warp of the grid.
 __device__ __forceinline__ void write_flags(const Params& p, const PrefixGroup* tab, int lane) {
+  for (int g = lane; g < p.own.groups.n; g += 32) {
+    const int lo = p.own.groups.cu[g], hi = p.own.groups.cu[g + 1];
+    if (p.own.err && (lo < 0 || hi < lo || hi > p.own.batch)) atomicCAS(p.own.err, 0, LA_DEVERR_PREFIX);
+  }
   for (int b = lane; b < p.own.batch; b += 32) {
     int block0;
     const int own = decode::own_keys<true>(p.own, tab, b, &block0);
@@ -841,8 +900,6 @@ __device__ __forceinline__ void write_flags(const Params& p, const PrefixGroup* 
   }
 }
 
-// kOwnStages: pipeline stages of the decode warps.
-template <int kOwnStages>
 __global__ void __launch_bounds__(kThreads, 1)
     shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap own_q,
@@ -861,10 +918,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   Plan& plan = *reinterpret_cast<Plan*>(smem + kOffPlan);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int wg = warp >> 2;
 
   // Barriers and tensor memory: nothing that a kernel before this one writes.
-  if (threadIdx.x == 32) {
+  if (warp == kWarpSetup && lane == 0) {
     mbar_init(bars.q_full(), 1);
     mbar_init(bars.q_empty(), 1);
     for (int i = 0; i < kStages; ++i) {
@@ -876,9 +932,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bars.s_free() + i, 1);
       mbar_init(bars.p_full() + i, 128);
       mbar_init(bars.o_empty() + i, 128);
-      mbar_init(bars.st_full() + i, 128);
-      mbar_init(bars.st_empty() + i, 128);
     }
+    mbar_init(bars.planned(), 1);
+    mbar_init(bars.checked(), 1);
+    mbar_init(bars.done(), 8);
     for (int s = 0; s < kOwnStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], decode::kCWarps);
@@ -887,12 +944,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(mg_empty, p.own.hkv);
     fence_barrier_init();
   }
-  if (warp == 2) reinterpret_cast<uint32_t*>(smem + kOffZero)[lane] = 0u;
-  if (warp == 12) {
+  if (warp == kWarpSetup) reinterpret_cast<uint32_t*>(smem + kOffZero)[lane] = 0u;
+  if (warp == kWarpProduct) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  if (warp == 13 && lane == 0) {
+  if (warp == kWarpLoad && lane == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -900,73 +957,145 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&own_k);
     tma_prefetch_desc(&own_v);
   }
-  grid_dependency_wait();
-  grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
-  if (warp == 0) {
-    const Plan r = make_plan(p, tab, lane);
-    if (lane == 0) plan = r;
-  }
+  // The plan is made before the wait for the kernel in front, from the lengths
+  // and groups as they are, and checked after it; if they changed, it is made
+  // again. Beyond 256 rows or 32 groups it is made after the wait.
+  const bool early = p.own.batch <= 256 && p.own.groups.n <= 32;
+  volatile int* stale = reinterpret_cast<volatile int*>(smem + kOffStale);
+  Seen in;
+  if (warp == kWarpPlan && early) in = read_inputs(p, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int P = plan.P;
-  const bool shares = static_cast<int>(blockIdx.x) < P;
-  if (warp == 12 && !shares) tmem_dealloc(tmem, kTmemCols);
-  if (!shares) {
-    if (wg < 2) {
-      regs_inc<kRegConsume>();
+  if (warp == kWarpPlan) {
+    if (!early) {
+      grid_dependency_wait();
+      in = read_inputs(p, lane);
+    }
+    for (int round = 0; round < 2; ++round) {
+      const Plan r = make_plan(p, tab, in, lane);
+      if (lane == 0) {
+        plan = r;
+        mbar_arrive(bars.planned());
+      }
+      grid_dependency_wait();
+      grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
+      if (round == 1) break;
+      bool same = true;
+      if (early) {
+        const Seen now = read_inputs(p, lane);
+        same = now.lo == in.lo && now.hi == in.hi && now.len == in.len;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) same &= now.raw[i] == in.raw[i];
+        same = __all_sync(0xffffffffu, same);
+        in = now;
+      }
+      if (lane == 0) {
+        *stale = !same;
+        mbar_arrive(bars.checked());
+      }
+      if (same) break;
+      named_sync(1, kThreads);  // everyone is done with the plan that was stale
+    }
+    if (blockIdx.x == 0) write_flags(p, tab, lane);
+    return;
+  }
+  if (warp == kWarpSetup) {  // no more work; takes part where everyone has to
+    if (wait_warp(p, bars.checked(), 0) && *stale) named_sync(1, kThreads);
+    return;
+  }
+  // The plan; `walk` goes by it, `look` reads by it from global memory before
+  // the check is back. All the warps that wait here do so a second time if the
+  // plan was stale.
+  auto begin = [&](auto walk, auto look) -> bool {
+    for (uint32_t round = 0;; ++round) {
+      if (!wait_warp(p, bars.planned(), round)) return false;
+      walk();
+      grid_dependency_wait();
+      look();
+      if (round == 1) return true;
+      if (!wait_warp(p, bars.checked(), 0)) return false;
+      if (!*stale) return true;
+      named_sync(1, kThreads);
+    }
+  };
+
+  if (warp < 8) {
+    // Both parts' warps make the dry round; those of a CTA for the rows' own
+    // keys go on as consumers.
+    bool own = false;
+    softmax_warp(p, tab, plan, smem, bars, tmem, warp >> 2, warp, lane, [&]() -> bool {
+      if (!begin([] {}, [] {})) return false;
+      own = !plan.shared;
+      return !own;
+    });
+    if (own)
       decode::consume<kOwnStages, true>(p.own, smem + kCtrlBytes, full, empty,
                                         reinterpret_cast<const decode::StageDesc*>(smem + kOffDesc), smem + kOffZero,
                                         mg_full, mg_empty,
                                         reinterpret_cast<float*>(smem + kCtrlBytes + kOwnStages * p.own.stage_bytes),
                                         plan.u1 - plan.u0, warp, lane);
-    } else if (wg == 2) {
-      regs_dec<kRegLoad>();
-      if (warp < decode::kCWarps + 2 && plan.u1 > plan.u0) {
-        decode::Windows<true> w;
-        w.tab = tab;
-        w.load_swin(p.own, lane, plan.at);
-        w.load_bwin(p.own, lane, plan.at, static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
-        decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
-                                          reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), w, plan.u0,
-                                          plan.u1 - plan.u0, plan.at, plan.before, static_cast<int>(blockIdx.x) - P,
-                                          warp - decode::kCWarps, 2, lane);
-      }
-    } else {
-      regs_dec<kRegIdle>();
-      if (warp == 15 && blockIdx.x == 0) write_flags(p, tab, lane);
-    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars.done());
     return;
   }
-  if (wg < 2) {
-    regs_inc<kRegSoftmax>();
-    softmax_warp(p, tab, plan, smem, bars, tmem, wg, warp, lane);
-  } else if (wg == 2) {
-    regs_dec<kRegStore>();
-    store_warp(p, tab, plan, smem, bars, tmem, warp, lane);
-  } else {
-    regs_dec<kRegOther>();
-    if (warp == 12) product_warp(p, tab, plan, smem, bars, tmem, lane);
-    if (warp == 15 && blockIdx.x == 0) write_flags(p, tab, lane);
-    if (warp == 13) load_warp(tm_q, tm_k, tm_v, p, tab, plan, smem, bars, lane);
+  // Warps 8 and 9: products and loads of the shared part, or both loads of the
+  // rows' own keys.
+  decode::Windows<true> win;
+  Walk w;
+  Segment e{};
+  Pages pages;
+  bool work = false;
+  const bool ok = begin(
+      [&] {
+        if (plan.shared) {
+          walk_start(p, tab, plan, w);
+          work = walk_next(p, tab, w, e);
+        }
+      },
+      [&] {
+        if (plan.shared) {
+          if (work && warp == kWarpLoad) pages.start(p, e, lane);
+        } else if (plan.u1 > plan.u0) {
+          win.tab = tab;
+          win.load_swin(p.own, lane, plan.at);
+          win.load_bwin(p.own, lane, plan.at,
+                        static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
+        }
+      });
+  if (ok) {
+    if (!plan.shared) {
+      if (plan.u1 > plan.u0)
+        decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
+                                          reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), win, plan.u0,
+                                          plan.u1 - plan.u0, plan.at, plan.before, plan.c, warp - decode::kCWarps, 2,
+                                          lane);
+    } else if (warp == kWarpLoad) {
+      load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, work, pages, lane);
+    } else {
+      product_warp(p, tab, smem, bars, tmem, w, e, work, lane);
+    }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 12) {
+  if (warp == kWarpProduct) {
+    // tensor memory is read by the eight warps until they are through
+    wait_warp(p, bars.done(), 0);
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
 }
 
 // ------------------------------------------------------------------ combine
-// A warp per (row, query head), lane l owning dims 4l..4l+3. The row's parts
-// are those of its group's item, one per CTA that had a segment of it (two
-// where the accumulators took alternate key tiles), and those of its own
-// keys. Up to 32 parts per round, one per lane: the weights come from a warp
-// maximum, the O rows are read 16 at a time, the first 16 together with the
-// logarithms. Bound by the latency of its three dependent reads.
-constexpr int kCombineBatch = 16;
+// A CTA per (row, query head); its four warps take every fourth run of 16 of
+// the row's parts and the first joins the warps' results. Lane l owns dims
+// 4l..4l+3. The row's parts are those of its group's item, one per CTA that
+// had a segment of it (two where the accumulators took alternate key tiles),
+// and those of its own keys. In a run the weights come from a maximum over
+// the lanes that hold the logarithms, and the O rows are requested together
+// with them. Bound by the latency of its three dependent reads (one row over
+// 148 parts in one warp took 20 us).
+constexpr int kRun = 16;
 constexpr int kCombineWarps = 4;
 
 struct CombineParams {
@@ -985,14 +1114,14 @@ struct CombineParams {
 };
 
 __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const CombineParams p) {
-  const int b = blockIdx.x;
-  const int hh = blockIdx.y * static_cast<int>(blockDim.x >> 5) + static_cast<int>(threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  __shared__ float4 s_acc[kCombineWarps - 1][32];
+  __shared__ float2 s_ml[kCombineWarps - 1];
+  const int b = blockIdx.x, hh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = hh / p.group;
   const float NEG_INF = -__int_as_float(0x7f800000);
   grid_dependency_wait();
   grid_launch_dependents();
-  if (hh >= p.hq) return;
-  const int h = hh / p.group;
   const int flags = p.flags[b];
   const int2 rp = p.row_parts[b];
   const int4 it = p.items[static_cast<long long>(b) * p.hkv + h];
@@ -1005,8 +1134,8 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
   const int n = pn + own;
   float m = NEG_INF, l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int e0 = 0; e0 < n; e0 += 32) {
-    const int x = e0 + lane;
+  for (int e0 = warp * kRun; e0 < n; e0 += kCombineWarps * kRun) {
+    const int x = e0 + (lane & (kRun - 1));
     int row = 0;
     if (x < pn)
       row = it.x + hh - h * p.group + (it.y ? (x >> 1) * 2 * kRows + (x & 1) * it.y : x * 2 * kRows);
@@ -1014,15 +1143,13 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
       row = p.own0 + (b + rp.x + x - pn) * p.hq + hh;
     row = min(max(row, 0), p.rows - 1);
     const float ls = x < n ? p.part_lse[row] : NEG_INF;
-    const int nr = min(n - e0, 32);
-    int su[kCombineBatch];
-    float4 ov[kCombineBatch];
+    float4 ov[kRun];
 #pragma unroll
-    for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, k);
-#pragma unroll
-    for (int k = 0; k < kCombineBatch; ++k)
-      ov[k] = k < nr ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < kRun; ++k) {
+      const int r = __shfl_sync(0xffffffffu, row, k);
+      ov[k] = e0 + k < n ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(r) * kD + lane * 4)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     // A part without keys has -inf and is left out by a test, never by a
     // weight of 0, so whatever its row holds does not count; NaN counts.
     const bool use = x < n && ls != NEG_INF;
@@ -1030,39 +1157,48 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
     if (usem == 0) continue;
     float mr = use ? ls : NEG_INF;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
+    for (int o = kRun / 2; o > 0; o >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
     const float mn = fmaxf(m, mr);
     const float a = ex2(m - mn);
     const float wl = use ? ex2(ls - mn) : 0.f;
     float ws = wl;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+    for (int o = kRun / 2; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
     l = l * a + ws;
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] *= a;
     m = mn;
-#pragma unroll 1
-    for (int j0 = 0; j0 < nr; j0 += kCombineBatch) {
-      if (j0 > 0) {
 #pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k) su[k] = __shfl_sync(0xffffffffu, row, (j0 + k) & 31);
-#pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k)
-          ov[k] = j0 + k < nr
-                      ? *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(su[k]) * kD + lane * 4)
-                      : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < kCombineBatch; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, wl, (j0 + k) & 31);
-        if (j0 + k < nr && ((usem >> ((j0 + k) & 31)) & 1u)) {
-          acc[0] += wk * ov[k].x;
-          acc[1] += wk * ov[k].y;
-          acc[2] += wk * ov[k].z;
-          acc[3] += wk * ov[k].w;
-        }
+    for (int k = 0; k < kRun; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, wl, k);
+      if ((usem >> k) & 1u) {
+        acc[0] += wk * ov[k].x;
+        acc[1] += wk * ov[k].y;
+        acc[2] += wk * ov[k].z;
+        acc[3] += wk * ov[k].w;
       }
     }
+  }
+  if (n > kRun) {  // the other warps' results, in their order
+    if (warp > 0) {
+      s_acc[warp - 1][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (lane == 0) s_ml[warp - 1] = make_float2(m, l);
+    }
+    __syncthreads();
+  }
+  if (warp > 0) return;
+  for (int w = 1; w * kRun < n && w < kCombineWarps; ++w) {
+    const float2 ml = s_ml[w - 1];
+    const float4 o = s_acc[w - 1][lane];
+    if (ml.y == 0.f) continue;
+    const float mn = fmaxf(m, ml.x);
+    const float a = l == 0.f ? 0.f : ex2(m - mn), c = ex2(ml.x - mn);
+    acc[0] = acc[0] * a + o.x * c;
+    acc[1] = acc[1] * a + o.y * c;
+    acc[2] = acc[2] * a + o.z * c;
+    acc[3] = acc[3] * a + o.w * c;
+    l = l * a + ml.y * c;
+    m = mn;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint2 v;
@@ -1099,11 +1235,8 @@ static Workspace workspace_of(int64_t batch, int hq, int hkv, int64_t grid) {
 
 int prefix_init(int device) {
   (void)device;
-  const int lim = 227 * 1024;
-  cudaError_t e =
-      cudaFuncSetAttribute(prefix::shared_prefix_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(prefix::shared_prefix_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, lim);
+  cudaError_t e = cudaFuncSetAttribute(prefix::shared_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       227 * 1024);
   cudaFuncAttributes a;
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, prefix::combine_kernel);
   return cuda_status(e);
@@ -1167,7 +1300,7 @@ extern "C" int la_paged_decode_shared_prefix(
   // steps of all groups and units of 256 rows are counted in 32 bits
   const int64_t key_tiles = (groups.cap + kKeys - 1) / kKeys, most_groups = num_groups < batch ? num_groups : batch;
   if (key_tiles * num_kv_heads * (batch / (2 * per_tile) + most_groups) > 0x7fffffffLL ||
-      256 * (groups.cap / call.p.tc + 1) > 0x7fffffffLL)
+      256 * (groups.cap / call.p.tc + 1) > 0x7fffffffLL || batch > (1 << 24))
     return LA_ERR_UNSUPPORTED;
 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1181,6 +1314,7 @@ extern "C" int la_paged_decode_shared_prefix(
   call.p.row_parts = reinterpret_cast<int*>(ws + w.parts);
   p.own = call.p;
   p.per_tile = per_tile;
+  p.tile_magic = static_cast<uint32_t>(((1ull << 32) + per_tile - 1) / per_tile);
   p.box_keys = kKeys;
   while (block_size % p.box_keys) p.box_keys >>= 1;
 
@@ -1200,12 +1334,11 @@ extern "C" int la_paged_decode_shared_prefix(
     if ((st = encode_tensor_map_bf16(&tk, k_cache, 4, dims, strides, box, true)) != LA_OK) return st;
     if ((st = encode_tensor_map_bf16(&tv, v_cache, 4, dims, strides, box, true)) != LA_OK) return st;
   }
-  size_t smem = 0;
-  const int stages = decode::stages_for(call.p.stage_bytes, kCtrlBytes + call.merge_bytes, &smem);
-  if (stages == 0) return LA_ERR_UNSUPPORTED;
-  if (smem < kSmemBytes) smem = kSmemBytes;
-  st = cuda_status(launch_pdl(stages == 3 ? shared_prefix_kernel<3> : shared_prefix_kernel<2>, dim3(grid),
-                              dim3(kThreads), smem, stream, tq, tk, tv, call.q, call.k, call.v, call.k1, call.v1, p));
+  const size_t own = kCtrlBytes + static_cast<size_t>(kOwnStages) * call.p.stage_bytes + call.merge_bytes + 1024;
+  const size_t smem = own > kSmemBytes ? own : kSmemBytes;
+  if (smem > 227 * 1024) return LA_ERR_UNSUPPORTED;
+  st = cuda_status(launch_pdl(shared_prefix_kernel, dim3(grid), dim3(kThreads), smem, stream, tq, tk, tv, call.q, call.k,
+                              call.v, call.k1, call.v1, p));
   if (st != LA_OK) return st;
 
   CombineParams c;
@@ -1224,7 +1357,5 @@ extern "C" int la_paged_decode_shared_prefix(
   c.out_bs = out_batch_stride;
   c.out_hs = out_head_stride;
   c.lse = softmax_lse;
-  const int warps = num_q_heads < kCombineWarps ? num_q_heads : kCombineWarps;
-  return cuda_status(launch_pdl(combine_kernel, dim3(batch, (num_q_heads + warps - 1) / warps), dim3(32 * warps), 0,
-                                stream, c));
+  return cuda_status(launch_pdl(combine_kernel, dim3(batch, num_q_heads), dim3(32 * kCombineWarps), 0, stream, c));
 }
