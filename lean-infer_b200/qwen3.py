@@ -12,6 +12,9 @@ confined to how the work is launched:
     instead of build_rope per forward (model.py:98);
   * decode attention (model.py:60-67) is flash_attn_with_kvcache from this
     package; prefill attention (model.py:56-57) is flash_attn_varlen_func;
+  * decode of rows that share a prompt's blocks (forked sequences, which the
+    reference does not have) is flash_attn_with_shared_prefix, where the
+    caller names the groups (prefix=);
   * each residual add and the RMSNorm after it are one launch
     (add_rms_norm), and SiLU(gate) * up is one launch (silu_mul);
   * the greedy next token, logits[:, -1].argmax(-1)
@@ -104,8 +107,10 @@ class Qwen3Attention(nn.Module):
 
     def attend(self, x: torch.Tensor, cache: BlockCache, layer: int, block_tables: torch.Tensor, pos: torch.Tensor,
                cache_seqlens: torch.Tensor | None, rope, cu_seqlens: torch.Tensor | None = None,
-               max_seqlen: int = 0) -> torch.Tensor:
-        """Attention output [T, hq*D] before o_proj. x: [T, hidden]."""
+               max_seqlen: int = 0, prefix: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """Attention output [T, hq*D] before o_proj. x: [T, hidden]. prefix:
+        decode rows that share blocks, (prefix_lens, cu_prefix_rows) of
+        flash_attn_with_shared_prefix."""
         T = x.shape[0]
         D = self.cfg.head_dim
         qkv = self.qkv_proj(x)
@@ -116,8 +121,12 @@ class Qwen3Attention(nn.Module):
         if cache_seqlens is not None:  # decode: one token per sequence
             q = fai.qk_norm_rope_paged_write(q, k, v, self.q_norm, self.k_norm, rope[0], rope[1], pos, block_tables,
                                              kc, vc, eps=self.cfg.rms_norm_eps)
-            o = fai.flash_attn_with_kvcache(q.view(T, 1, self.hq, D), kc, vc, cache_seqlens=cache_seqlens,
-                                            block_table=block_tables, causal=True, num_splits=1)
+            if prefix is not None:
+                o = fai.flash_attn_with_shared_prefix(q.view(T, 1, self.hq, D), kc, vc, cache_seqlens, block_tables,
+                                                      *prefix)
+            else:
+                o = fai.flash_attn_with_kvcache(q.view(T, 1, self.hq, D), kc, vc, cache_seqlens=cache_seqlens,
+                                                block_table=block_tables, causal=True, num_splits=1)
         else:  # prefill of packed prompts starting at pos
             k_out = torch.empty_like(k)
             q = fai.qk_norm_rope_paged_write(q, k, v, self.q_norm, self.k_norm, rope[0], rope[1], pos, block_tables,
@@ -125,9 +134,10 @@ class Qwen3Attention(nn.Module):
             o = fai.flash_attn_varlen_func(q, k_out, v, cu_seqlens, cu_seqlens, max_seqlen, max_seqlen, causal=True)
         return o.reshape(T, self.hq * D)
 
-    def forward(self, x, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens=None, max_seqlen=0):
+    def forward(self, x, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens=None, max_seqlen=0,
+                prefix=None):
         return self.o_proj(self.attend(x, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens,
-                                       max_seqlen))
+                                       max_seqlen, prefix))
 
 
 class Qwen3MLP(nn.Module):
@@ -151,12 +161,12 @@ class Qwen3DecoderLayer(nn.Module):
         self.eps = cfg.rms_norm_eps
 
     def forward(self, h, x, next_norm, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens=None,
-                max_seqlen=0):
+                max_seqlen=0, prefix=None):
         """h: residual stream [T, hidden]; x = RMSNorm(h) * input_layernorm
         (produced by the previous layer's last fused add). Returns the new h
         and RMSNorm(h) * next_norm (the next layer's input norm, or the
         model's final norm)."""
-        a = self.self_attn(x, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens, max_seqlen)
+        a = self.self_attn(x, cache, layer, block_tables, pos, cache_seqlens, rope, cu_seqlens, max_seqlen, prefix)
         h, x = add_rms_norm(h, a, self.post_attention_layernorm, self.eps)
         return add_rms_norm(h, self.mlp(x), next_norm, self.eps)
 
@@ -180,8 +190,9 @@ class Qwen3ForCausalLM(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, cache: BlockCache, block_tables: torch.Tensor, pos: torch.Tensor,
                 cache_seqlens: torch.Tensor | None, cu_seqlens: torch.Tensor | None = None,
-                max_seqlen: int = 0) -> torch.Tensor:
-        """Decode: input_ids [B, 1], cache_seqlens [B] -> logits [B, 1, vocab].
+                max_seqlen: int = 0, prefix: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """Decode: input_ids [B, 1], cache_seqlens [B] -> logits [B, 1, vocab];
+        prefix: (prefix_lens [G], cu_prefix_rows [G+1]) where rows share blocks.
         Prefill: input_ids [T] packed, cu_seqlens [S+1] -> logits [T, vocab].
         The rope table must already cover every position (call rope() before
         capturing a graph)."""
@@ -192,7 +203,7 @@ class Qwen3ForCausalLM(nn.Module):
         _, x = add_rms_norm(h, None, self.layers[0].input_layernorm, eps)
         for i, layer in enumerate(self.layers):
             nxt = self.layers[i + 1].input_layernorm if i + 1 < len(self.layers) else self.norm
-            h, x = layer(h, x, nxt, cache, i, block_tables, pos, cache_seqlens, rope, cu_seqlens, max_seqlen)
+            h, x = layer(h, x, nxt, cache, i, block_tables, pos, cache_seqlens, rope, cu_seqlens, max_seqlen, prefix)
         logits = F.linear(x, self.embed_tokens.weight)  # x = final RMSNorm(h) * norm
         return logits.view(input_ids.shape[0], -1, logits.shape[-1]) if cache_seqlens is not None else logits
 
@@ -226,6 +237,36 @@ def staging_bytes(n_slots: int, max_blocks: int) -> int:
     return 20 * n_slots + 4 * n_slots * max_blocks
 
 
+def prefix_views(buf: torch.Tensor, groups: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(prefix_lens [groups] i32, cu_prefix_rows [groups + 1] i32) as views of
+    one uint8 buffer of prefix_bytes(groups) bytes."""
+    assert buf.dtype == torch.uint8 and buf.numel() == prefix_bytes(groups)
+    return buf[: 4 * groups].view(torch.int32), buf[4 * groups:].view(torch.int32)
+
+
+def prefix_bytes(groups: int) -> int:
+    return 4 * (2 * groups + 1)
+
+
+def stage_prefix(lens: torch.Tensor, cu: torch.Tensor, prefix, rows: int) -> None:
+    """Fill host buffers lens [G], cu [G + 1] with the groups of a step, as
+    shared_prefix_groups returns them (None: no rows share), the rest of the
+    groups empty."""
+    given_lens, given_cu = ([], [0]) if prefix is None else prefix
+    given_lens, given_cu = torch.as_tensor(given_lens, dtype=torch.int32), torch.as_tensor(given_cu, dtype=torch.int32)
+    n = given_lens.numel()
+    if given_cu.numel() != n + 1:
+        raise ValueError("cu_prefix_rows must have one entry more than prefix_lens")
+    if n > lens.numel():
+        raise ValueError(f"{n} prefix groups, the graph was made for {lens.numel()}")
+    if bool((given_cu.diff() < 0).any()) or int(given_cu[0]) < 0 or int(given_cu[-1]) > rows:
+        raise ValueError(f"cu_prefix_rows must ascend within the {rows} rows")
+    lens[:n] = given_lens
+    lens[n:] = 0
+    cu[: n + 1] = given_cu
+    cu[n + 1:] = given_cu[-1]
+
+
 class DecodeGraph:
     """Fixed-B decode step captured in a CUDA graph — the engine's DecodeGraph
     (leaninfer/engine/llm_engine.py:23-86): pinned host staging buffers,
@@ -234,16 +275,23 @@ class DecodeGraph:
     rows get pos 0, ctx 1 and block 0 (the trash block). The four host
     buffers are views of one pinned allocation and the four device buffers
     views of one device allocation with the same layout, so a step's inputs
-    go up in a single copy."""
+    go up in a single copy. With prefix_groups, rows may share blocks
+    (BlockCache.fork): a step names up to that many groups of them
+    (stage(prefix=)), whose prefixes are then read once for all their rows."""
 
-    def __init__(self, model: Qwen3ForCausalLM, cache: BlockCache, n_slots: int, max_blocks: int) -> None:
+    def __init__(self, model: Qwen3ForCausalLM, cache: BlockCache, n_slots: int, max_blocks: int,
+                 prefix_groups: int = 0) -> None:
         self.model, self.cache = model, cache
         dev = cache.device
         nbytes = staging_bytes(n_slots, max_blocks)
-        self._host_buf = torch.zeros(nbytes, dtype=torch.uint8, pin_memory=True)
-        self._dev_buf = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        self.host_ids, self.host_pos, self.host_ctx, self.host_bt = staging_views(self._host_buf, n_slots, max_blocks)
-        self.ids, self.pos, self.ctx, self.bt = staging_views(self._dev_buf, n_slots, max_blocks)
+        total = nbytes + (prefix_bytes(prefix_groups) if prefix_groups else 0)
+        self._host_buf = torch.zeros(total, dtype=torch.uint8, pin_memory=True)
+        self._dev_buf = torch.zeros(total, dtype=torch.uint8, device=dev)
+        self.host_ids, self.host_pos, self.host_ctx, self.host_bt = staging_views(self._host_buf[:nbytes], n_slots,
+                                                                                  max_blocks)
+        self.ids, self.pos, self.ctx, self.bt = staging_views(self._dev_buf[:nbytes], n_slots, max_blocks)
+        self.host_prefix = prefix_views(self._host_buf[nbytes:], prefix_groups) if prefix_groups else None
+        self.prefix = prefix_views(self._dev_buf[nbytes:], prefix_groups) if prefix_groups else None
         self.host_ctx.fill_(1)
         self.ctx.fill_(1)
         self.graph: torch.cuda.CUDAGraph | None = None
@@ -253,10 +301,10 @@ class DecodeGraph:
 
     @property
     def h2d_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.host_ids, self.host_pos, self.host_bt, self.host_ctx))
+        return self._host_buf.numel()
 
     def _forward(self):
-        logits = self.model(self.ids, self.cache, self.bt, self.pos, self.ctx)
+        logits = self.model(self.ids, self.cache, self.bt, self.pos, self.ctx, prefix=self.prefix)
         return logits, argmax_rows(logits[:, -1])
 
     def capture(self) -> None:
@@ -270,8 +318,13 @@ class DecodeGraph:
         with torch.cuda.graph(self.graph):
             self.logits, self.next_tokens = self._forward()
 
-    def stage(self, ids, pos, bt, ctx) -> None:
-        """Fill the pinned host buffers (numpy-style views, as the engine does)."""
+    def stage(self, ids, pos, bt, ctx, prefix=None) -> None:
+        """Fill the pinned host buffers (numpy-style views, as the engine does).
+        prefix: (prefix_lens, cu_prefix_rows) of the rows that share blocks."""
+        if self.host_prefix is not None:
+            stage_prefix(*self.host_prefix, prefix, self.host_ctx.numel())
+        elif prefix is not None:
+            raise ValueError("the graph was made without prefix_groups")
         self.host_ids.copy_(ids)
         self.host_pos.copy_(pos)
         self.host_bt.zero_()
@@ -306,9 +359,11 @@ class BucketedDecodeGraph:
     masked — start position -1 and context 0 — so they write no cache slot
     (la_qk_norm_rope_paged_write skips them) and attend to nothing
     (la_paged_decode returns zeros): no trash block is needed and a small
-    batch does not pay for n_slots rows."""
+    batch does not pay for n_slots rows. With prefix_groups, active rows may
+    share blocks, as in DecodeGraph."""
 
-    def __init__(self, model: Qwen3ForCausalLM, cache: BlockCache, buckets, max_blocks: int) -> None:
+    def __init__(self, model: Qwen3ForCausalLM, cache: BlockCache, buckets, max_blocks: int,
+                 prefix_groups: int = 0) -> None:
         self.model, self.cache = model, cache
         self.buckets = sorted({int(b) for b in buckets})
         if not self.buckets or self.buckets[0] <= 0:
@@ -323,6 +378,10 @@ class BucketedDecodeGraph:
         self.pos = torch.full((n,), -1, dtype=torch.long, device=dev)
         self.bt = torch.zeros(n, max_blocks, dtype=torch.int32, device=dev)
         self.ctx = torch.zeros(n, dtype=torch.int32, device=dev)
+        self._host_prefix = torch.zeros(prefix_bytes(prefix_groups), dtype=torch.uint8, pin_memory=True)
+        self._dev_prefix = torch.zeros(prefix_bytes(prefix_groups), dtype=torch.uint8, device=dev)
+        self.host_prefix = prefix_views(self._host_prefix, prefix_groups) if prefix_groups else None
+        self.prefix = prefix_views(self._dev_prefix, prefix_groups) if prefix_groups else None
         self.graphs: dict[int, tuple] = {}
         self.bucket = n
         self.active = 0
@@ -335,10 +394,10 @@ class BucketedDecodeGraph:
         raise ValueError(f"{rows} active rows exceed the largest bucket {self.buckets[-1]}")
 
     def h2d_bytes(self, bucket: int) -> int:
-        return bucket * (8 + 8 + 4 + self.host_bt.shape[1] * 4)
+        return bucket * (8 + 8 + 4 + self.host_bt.shape[1] * 4) + (self._host_prefix.numel() if self.prefix else 0)
 
     def _forward(self, b: int):
-        logits = self.model(self.ids[:b], self.cache, self.bt[:b], self.pos[:b], self.ctx[:b])
+        logits = self.model(self.ids[:b], self.cache, self.bt[:b], self.pos[:b], self.ctx[:b], prefix=self.prefix)
         return logits, argmax_rows(logits[:, -1])
 
     def capture(self) -> None:
@@ -359,11 +418,16 @@ class BucketedDecodeGraph:
                 logits, nxt = self._forward(b)
             self.graphs[b] = (g, logits, nxt)
 
-    def stage(self, ids, pos, bt, ctx) -> int:
+    def stage(self, ids, pos, bt, ctx, prefix=None) -> int:
         """Stage the active rows (the first len(ids) rows) and mask the rest
-        of the chosen bucket; returns the bucket."""
+        of the chosen bucket; returns the bucket. prefix: (prefix_lens,
+        cu_prefix_rows) of the active rows that share blocks."""
         n = int(ids.shape[0])
         b = self.bucket_for(n)
+        if self.host_prefix is not None:
+            stage_prefix(*self.host_prefix, prefix, n)
+        elif prefix is not None:
+            raise ValueError("the graphs were made without prefix_groups")
         self.host_ids[:n].copy_(ids.view(n, 1))
         self.host_ids[n:b].zero_()
         self.host_pos[:n].copy_(pos)
@@ -385,6 +449,8 @@ class BucketedDecodeGraph:
         self.pos[:b].copy_(self.host_pos[:b], non_blocking=True)
         self.bt[:b].copy_(self.host_bt[:b], non_blocking=True)
         self.ctx[:b].copy_(self.host_ctx[:b], non_blocking=True)
+        if self.prefix is not None:
+            self._dev_prefix.copy_(self._host_prefix, non_blocking=True)
         g, _, nxt = self.graphs[b]
         g.replay()
         return nxt[: self.active].tolist()

@@ -192,3 +192,18 @@ def test_c_entries_check_arguments(pkg):
     assert prefix(q=null) == 1 and prefix(cu=null) == 1 and prefix(groups=-1) == 1 and prefix(scale=0.0) == 1
     assert prefix(bs=24) == 2 and prefix(d=64) == 2 and prefix(hq=72) == 2
     assert prefix(q=odd) == 3 and prefix(qs=2044) == 3
+
+
+def test_staged_prefix_groups(pkg):
+    from lean_infer_b200 import qwen3
+
+    buf = torch.full((qwen3.prefix_bytes(4),), 255, dtype=torch.uint8)
+    lens, cu = qwen3.prefix_views(buf, 4)
+    assert lens.shape == (4,) and cu.shape == (5,)
+    qwen3.stage_prefix(lens, cu, ([32, 64], [0, 3, 5]), 8)
+    assert lens.tolist() == [32, 64, 0, 0] and cu.tolist() == [0, 3, 5, 5, 5]
+    qwen3.stage_prefix(lens, cu, None, 8)
+    assert lens.tolist() == [0] * 4 and cu.tolist() == [0] * 5
+    for bad in (([1] * 5, list(range(6))), ([1], [0, 9]), ([1, 1], [0, 4, 2]), ([1], [0]), ([1], [-1, 2])):
+        with pytest.raises(ValueError):
+            qwen3.stage_prefix(lens, cu, bad, 8)
