@@ -34,8 +34,10 @@ __device__ __forceinline__ PrefixGroup group_from(const PrefixGroups& G, int fir
   r.keys = r.rows >= 2 ? blocks * G.block_size : 0;
   return r;
 }
+// Through L2 only: it may be read before the kernel in front is done, and no
+// stale line may stay in L1.
 __device__ __forceinline__ PrefixGroup load_group(const PrefixGroups& G, int g) {
-  return group_from(G, G.cu[g], G.cu[g + 1], G.lens[g]);
+  return group_from(G, __ldcg(G.cu + g), __ldcg(G.cu + g + 1), __ldcg(G.lens + g));
 }
 
 // From the CTA's table of all groups, where there is room for one.

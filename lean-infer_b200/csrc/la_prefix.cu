@@ -35,8 +35,8 @@
 // CTA, 12 warps. Shared part: 0-3 and 4-7 softmax of tile 0 and 1 (a thread
 // per row, the S row in registers), which store the segments' O as well, 8
 // issues the products, 9 the TMA loads; tensor memory holds S0 S1 O0 O1, 128
-// columns each, P over S. Own keys: 0-7 consume, 8 and 9 load. 10 makes the
-// plan, 11 sets the barriers up.
+// columns each, P over S. Own keys: 0-7 consume, 10 and 11 load. 10 makes the
+// plan.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -80,15 +80,15 @@ constexpr size_t kSmemBytes = kOffKV + kStages * kTile + 1024;  // + alignment t
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(kOffWalk + 8 * kWalkBytes <= kOffTable && kOffTable + kMaxGroups * sizeof(PrefixGroup) <= kCtrlBytes,
               "control area");
-// Warps behind the eight of softmax or consumers.
+// Warps behind the eight of softmax or consumers: two of the shared part, two
+// that load the rows' own keys, the first of which makes the plan.
 // Pipeline stages (of 64 KB) of the decode warps. What they keep in flight,
 // 128 KB on each SM, draws all that HBM has; the third stage that fits only
 // makes every load wait longer, and the shared part, whose CTAs keep less in
 // flight, waits with them (128 rows behind 2048 keys: 74 us with three, 61
 // with two).
 constexpr int kOwnStages = 2;
-constexpr int kWarpProduct = 8, kWarpLoad = 9;  // own keys: both load
-constexpr int kWarpPlan = 10, kWarpSetup = 11;
+constexpr int kWarpProduct = 8, kWarpLoad = 9, kWarpPlan = 10, kWarpSecond = 11;
 
 // The time model that divides the SMs (shared_ctas). Microseconds on a B200 at
 // ~1.9 GHz, fitted to the times of 15 calls with 2 to 146 CTAs for the shared
@@ -241,11 +241,17 @@ __device__ __forceinline__ int units8(const Params& p, const PrefixGroup* tab, c
   return sum;
 }
 
-// First of T steps or units of CTA c of G; T counts that fit are divided in 32
-// bits, in a fraction of the time.
-__device__ __forceinline__ long long part_start(int c, long long T, int G) {
-  if (T < (1 << 22)) return static_cast<unsigned>(c) * static_cast<unsigned>(T) / static_cast<unsigned>(G);
-  return c * T / G;
+// x / d for x < 2^16 and d < 2^10, rounded down: the quotient of x + 1/2 is at
+// least 1 / (2 d) away from a whole number, far more than its rounding.
+__device__ __forceinline__ int small_div(int x, float inv_d) {
+  return static_cast<int>((static_cast<float>(x) + 0.5f) * inv_d);
+}
+
+// First of T steps or units of CTA c of G: floor(c T / G).
+__device__ __forceinline__ long long part_start(int c, long long T, int G) { return c * T / G; }
+__device__ __forceinline__ int part_start(int c, int T, int G, float inv_G) {
+  const int q = T / G;
+  return c * q + small_div(c * (T - q * G), inv_G);
 }
 
 // CTAs of the shared part, an even number, from its steps, the rows' units and
@@ -255,20 +261,22 @@ __device__ __forceinline__ long long part_start(int c, long long T, int G) {
 // row tiles, whose loads are needed soonest, take f^3 as long, the others,
 // whose loads are twice as many, f^0.5. A CTA whose range is not within one
 // item has two segments to store.
-__device__ __forceinline__ int shared_ctas(const Params& p, long long pair_steps, long long single_steps,
-                                           long long units, int items, int grid, int lane) {
-  const float a = static_cast<float>(pair_steps), b = static_cast<float>(single_steps), u = static_cast<float>(units);
-  const float work = a * kPairUs + b * kSingleUs, unit = p.own.nsub > 1 ? kUnitMergedUs : kUnitUs;
-  const float loads = __fdividef(a + 2.f * b, work);  // 64 KB per us and CTA
+__device__ __forceinline__ int shared_ctas(const Params& p, float pair_steps, float single_steps, float units,
+                                           int items, int grid, int lane) {
+  const float a = pair_steps * kPairUs, b = single_steps * kSingleUs, steps = pair_steps + single_steps;
+  const float unit = p.own.nsub > 1 ? kUnitMergedUs : kUnitUs, own_work = units * unit;
+  const float loads = __fdividef(pair_steps + 2.f * single_steps, a + b) * kHbmUs;  // of one CTA, of HBM's rate
+  const float own_loads = __fdividef(kHbmUs, unit), per_item = __fdividef(1.f, static_cast<float>(items));
   float best = 3e38f;
   int at = 2;
+#pragma unroll 1
   for (int P = 2 + 2 * lane; P <= grid; P += 64) {
-    const float cs = fminf(static_cast<float>(P), a + b), co = fminf(static_cast<float>(grid - P), u);
-    const float f = fmaxf(1.f, (cs * loads + __fdividef(co, unit)) * kHbmUs);
-    const float shared = __fdividef(a * kPairUs * f * f * f + b * kSingleUs * sqrtf(f), cs) +
-                         (P % items ? kSegmentUs : 0.f);
-    const float own = u > 0.f ? (co > 0.f ? __fdividef(u * unit, co) : 1e38f) : 0.f;
-    const float t = fmaxf(shared, own);
+    const float x = static_cast<float>(P), cs = fminf(x, steps), co = fminf(static_cast<float>(grid - P), units);
+    const float f = fmaxf(1.f, cs * loads + co * own_loads);
+    // whole items per CTA or CTAs per item: P * per_item is whole up to rounding
+    const float y = x * per_item, odd = fabsf(y - rintf(y)) > 1e-3f ? kSegmentUs : 0.f;
+    const float t = fmaxf(__fdividef(a * f * f * f + b * sqrtf(f), cs) + odd,
+                          units > 0.f ? __fdividef(own_work, fmaxf(co, 1e-6f)) : 0.f);
     if (t < best) {
       best = t;
       at = P;
@@ -279,113 +287,141 @@ __device__ __forceinline__ int shared_ctas(const Params& p, long long pair_steps
   return static_cast<int>(__reduce_min_sync(0xffffffffu, __float_as_uint(best) == least ? at : 0x7fffffffu));
 }
 
-// One warp's work. tab: the table to fill, or null where the groups exceed it.
-// in: the first 256 rows and 32 groups.
+// The part that the CTA takes, and its number there. Neighbouring CTAs mostly
+// land on the two SMs of a TPC, next pairs on the same GPC. A pair has the same
+// part (two that stream load 114 GB/s together, one beside a tensor core CTA
+// ~48 GB/s while that one takes 1.3 times as long), and the pairs that stream
+// are spread evenly among the others. Q: CTAs that stream, an even number.
+__device__ __forceinline__ void take_part(Plan& r, int Q, int grid, bool any_shared) {
+  const int pairs = grid >> 1, pair = static_cast<int>(blockIdx.x >> 1), half = Q >> 1;
+  const float inv = __fdividef(1.f, static_cast<float>(pairs));
+  const int before = small_div(pair * half, inv);
+  r.shared = any_shared && (pair >= pairs || small_div((pair + 1) * half, inv) == before);
+  r.c = static_cast<int>(blockIdx.x);
+  if (any_shared) r.c = r.shared ? r.c - 2 * min(before, half) : 2 * before + (r.c & 1);
+  r.u0 = r.u1 = r.before = 0;
+  r.at = 0;
+}
+
+// One warp's work, for up to 256 rows and 32 groups: `in`, all in registers.
 __device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, const Seen& in, int lane) {
   const PrefixGroups& G = p.own.groups;
+  PrefixGroup grp{0, 0, 0};
+  Shape h{0, 0, 0, 0, 0};
+  if (lane < G.n) {
+    grp = group_from(G, in.lo, in.hi, in.len);
+    tab[lane] = grp;
+    if (grp.keys > 0) h = shape_of(p, grp);
+  }
+  const int mine = p.own.hkv * h.per_head;
+  const int S = warp_sum(mine), single = warp_sum(p.own.hkv * h.half);
+  const int items = warp_sum(h.tiles ? p.own.hkv * h.pairs : 0);
   int raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) raw[i] = in.raw[i];
-  // the shared part: steps, and key tiles that are read
-  long long S = 0, single = 0;
+  const int first = units8(p, tab, grp, true, lane, 0, raw);
+  const int U = warp_sum(first);
+  const int grid = static_cast<int>(gridDim.x);
+  const int Q = S > 0 ? (grid - shared_ctas(p, static_cast<float>(S - single), static_cast<float>(single),
+                                            static_cast<float>(U), items, grid, lane)) & ~1
+                      : grid;
+  Plan r;
+  take_part(r, Q, grid, S > 0);
+  // no more CTAs than units, so that a row's parts are those of consecutive ones
+  const int T = r.shared ? S : U, n = min(T, r.shared ? grid - Q : Q);
+  if (r.c >= n) return r;
+  const float inv = __fdividef(1.f, static_cast<float>(n));
+  const int u0 = part_start(r.c, T, n, inv);
+  r.u0 = u0;
+  r.u1 = part_start(r.c + 1, T, n, inv);
+  // the lane that holds the first one: a group each, or eight rows
+  const int incl = warp_scan(r.shared ? mine : first, lane);
+  const int src = __ffs(__ballot_sync(0xffffffffu, incl > u0)) - 1;
+  int at = 0, before = incl - (r.shared ? mine : first);
+  if (!r.shared) {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      found |= u0 < before + raw[i];
+      if (!found) {
+        before += raw[i];
+        at = i + 1;
+      }
+    }
+  }
+  r.at = __shfl_sync(0xffffffffu, r.shared ? lane : 8 * lane + at, src);
+  r.before = __shfl_sync(0xffffffffu, before, src);
+  return r;
+}
+
+// The same for any number of rows and groups. tab: the table to fill, or null
+// where the groups exceed it.
+__device__ __noinline__ Plan make_large_plan(const Params& p, PrefixGroup* tab, int lane) {
+  const PrefixGroups& G = p.own.groups;
+  int raw[8];
+  long long S = 0, single = 0, U = 0;
   int items = 0;
-  PrefixGroup grp{0, 0, 0};
+  const PrefixGroup none{0, 0, 0};
   for (int b = 0; b < G.n; b += 32) {
     const int g = b + lane;
-    int s = 0, s1 = 0, t = 0;
+    Shape h{0, 0, 0, 0, 0};
     if (g < G.n) {
-      const PrefixGroup r = b == 0 ? group_from(G, in.lo, in.hi, in.len) : load_group(G, g);
-      if (b == 0) grp = r;
+      const PrefixGroup r = load_group(G, g);
       if (tab) tab[g] = r;
-      if (r.keys > 0) {
-        const Shape h = shape_of(p, r);
-        s = p.own.hkv * h.per_head;
-        s1 = p.own.hkv * h.half;
-        t = p.own.hkv * h.pairs;
-      }
+      if (r.keys > 0) h = shape_of(p, r);
     }
-    S += warp_sum(s);
-    single += warp_sum(s1);
-    items += warp_sum(t);
+    S += warp_sum(p.own.hkv * h.per_head);
+    single += warp_sum(p.own.hkv * h.half);
+    items += warp_sum(h.tiles ? p.own.hkv * h.pairs : 0);
   }
   __syncwarp();
-  // the rows' own keys: units
-  const bool in_regs = G.n <= 32;
-  const int first = units8(p, tab, grp, in_regs, lane, 0, raw);
-  long long U = warp_sum(first);
-  for (int base = 256; base < G.batch; base += 256) {
-    int x[8];
-    load_lens8(p, lane, base, x);
-    U += warp_sum(units8(p, tab, grp, in_regs, lane, base, x));
+  for (int base = 0; base < G.batch; base += 256) {
+    load_lens8(p, lane, base, raw);
+    U += warp_sum(units8(p, tab, none, false, lane, base, raw));
   }
   const int grid = static_cast<int>(gridDim.x);
-  const int Q = S > 0 ? (grid - shared_ctas(p, S - single, single, U, items, grid, lane)) & ~1 : grid;
-  // Neighbouring CTAs mostly land on the two SMs of a TPC, next pairs on the
-  // same GPC. A pair has the same part (two that stream load 114 GB/s together,
-  // one beside a tensor core CTA ~48 GB/s while that one takes 1.3 times as
-  // long), and the pairs that stream are spread evenly among the others.
-  const int pairs = grid >> 1, pair = static_cast<int>(blockIdx.x >> 1), before = pair * (Q >> 1) / pairs;
+  const int Q = S > 0 ? (grid - shared_ctas(p, static_cast<float>(S - single), static_cast<float>(single),
+                                            static_cast<float>(U), items, grid, lane)) & ~1
+                      : grid;
   Plan r;
-  r.shared = S > 0 && (pair >= pairs || (pair + 1) * (Q >> 1) / pairs == before);
-  r.c = r.shared ? static_cast<int>(blockIdx.x) - 2 * min(before, Q >> 1) : 2 * before + static_cast<int>(blockIdx.x & 1);
-  r.u0 = r.u1 = r.before = 0;
-  r.at = 0;
-  if (r.shared) {
-    const int n = static_cast<int>(S < grid - Q ? S : grid - Q);
-    if (r.c < n) {
-      r.u0 = part_start(r.c, S, n);
-      r.u1 = part_start(r.c + 1, S, n);
+  take_part(r, Q, grid, S > 0);
+  const long long T = r.shared ? S : U;
+  const int most = r.shared ? grid - Q : Q, n = static_cast<int>(T < most ? T : most);
+  if (r.c >= n) return r;
+  r.u0 = part_start(r.c, T, n);
+  r.u1 = part_start(r.c + 1, T, n);
+  long long acc = 0;
+  const int count = r.shared ? G.n : G.batch, stride = r.shared ? 32 : 256;
+  for (int base = 0; base < count; base += stride) {
+    int sum = 0;
+    if (r.shared) {
+      if (base + lane < G.n) sum = steps_of(p, prefix_group(G, tab, base + lane));
+    } else {
+      load_lens8(p, lane, base, raw);
+      sum = units8(p, tab, none, false, lane, base, raw);
     }
-    long long acc = 0;
-    for (int b = 0; b < G.n; b += 32) {  // the group of the first step
-      const int s = b + lane < G.n ? steps_of(p, prefix_group(G, tab, b + lane)) : 0;
-      const int incl = warp_scan(s, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        r.at = b + src;
-        r.before = acc + __shfl_sync(0xffffffffu, incl - s, src);
-        break;
-      }
-      acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-  } else {
-    // no more CTAs than units, so that a row's parts are those of consecutive ones
-    const int n = static_cast<int>(U < Q ? U : Q);
-    if (r.c < n) {
-      r.u0 = part_start(r.c, U, n);
-      r.u1 = part_start(r.c + 1, U, n);
-      long long acc = 0;
-      for (int base = 0; base < G.batch; base += 256) {  // the row of the first unit
-        int sum = first;
-        if (base > 0) {
-          load_lens8(p, lane, base, raw);
-          sum = units8(p, tab, grp, in_regs, lane, base, raw);
-        }
-        const int incl = warp_scan(sum, lane);
-        const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
-        if (hit) {
-          const int src = __ffs(hit) - 1;
-          int at = 0;
-          long long before = acc + incl - sum;
-          if (lane == src) {
-            bool found = false;
+    const int incl = warp_scan(sum, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > r.u0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      int at = 0;
+      long long before = acc + incl - sum;
+      if (!r.shared) {
+        bool found = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              found |= r.u0 < before + raw[i];
-              if (!found) {
-                before += raw[i];
-                at = i + 1;
-              }
-            }
+        for (int i = 0; i < 8; ++i) {
+          found |= r.u0 < before + raw[i];
+          if (!found) {
+            before += raw[i];
+            at = i + 1;
           }
-          r.at = base + 8 * src + __shfl_sync(0xffffffffu, at, src);
-          r.before = __shfl_sync(0xffffffffu, before, src);
-          break;
         }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
       }
+      r.at = base + __shfl_sync(0xffffffffu, r.shared ? lane : 8 * lane + at, src);
+      r.before = __shfl_sync(0xffffffffu, before, src);
+      break;
     }
+    acc += __shfl_sync(0xffffffffu, incl, 31);
   }
   return r;
 }
@@ -505,13 +541,8 @@ __device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32
 }
 
 // Softmax of tile t and the segments' results, four warps, a thread per row.
-// begin() brings the plan: called once, after a first round over whatever the
-// S columns hold, which writes nothing. That round fetches the code while the
-// lengths, and then the first tiles, are on their way; fetched line by line as
-// the first tile ran, beside CTAs that fill HBM, it took up to 16 us.
-template <typename Begin>
 __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
-                                             Bars bars, uint32_t tmem, int t, int warp, int lane, Begin begin) {
+                                             Bars bars, uint32_t tmem, int t, int warp, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* s_full = bars.s_full();
   uint64_t* s_free = bars.s_free();
@@ -538,25 +569,25 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
     return more;
   };
   uint32_t seen = 0;  // S tiles
-  bool ok = true, dry = true;
-  if (lane == 0) {  // the first round's segment: a full key tile, rows of which none is stored
-    e = Segment{};
-    e.two = e.tiles = 1;
-    e.keys = kKeys;
+  bool ok = true;
+  {
+    Walk x;
+    walk_start(p, tab, plan, x);
+    if (lane == 0) w = x;
+    __syncwarp();
   }
-  __syncwarp();
-  while (dry || (ok && next())) {
+  while (ok && next()) {
     const int n = tiles_of(e, t);
-    const int rows = dry ? 0 : rows_of(p, e, t);
+    const int rows = rows_of(p, e, t);
     const int row0 = e.row0 + t * rows_of(p, e, 0);
     if (n == 0) {  // a single key tile: none for the second accumulator
       if (row < rows) p.part_lse[row0 + row] = NEG_INF;
       continue;
     }
-    const bool active = dry || quarter * 32 < rows;  // rows of this warp
+    const bool active = quarter * 32 < rows;  // rows of this warp
     float m = NEG_INF, l = 0.f;
     for (int j = 0; j < n; ++j, ++seen) {
-      if (!dry && !(ok = wait_all(&s_full[t], seen & 1))) break;
+      if (!(ok = wait_all(&s_full[t], seen & 1))) break;
       if (!active) {
         mbar_arrive(&p_full[t]);
         continue;
@@ -598,27 +629,6 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       uint64_t acc2[4];
 #pragma unroll
       for (int a = 0; a < 4; ++a) acc2[a] = 0ull;
-      // P rounded to bf16, the type of V, for the product; l sums it unrounded.
-#pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) {
-        float pk[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const uint64_t y2 =
-              f2_fma(f2_pack(sv[2 * c2 + (x >> 4)][(x & 15) * 2], sv[2 * c2 + (x >> 4)][(x & 15) * 2 + 1]), sl2x2, negm2);
-          float e0, e1;
-          f2_unpack(y2, e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
-          pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
-        }
-        if (!dry) tmem_st32(taddr + colS + c2 * 32, pk);
-      }
-      float ps[8];
-#pragma unroll
-      for (int a = 0; a < 4; ++a) f2_unpack(acc2[a], ps[2 * a], ps[2 * a + 1]);
-      l = l * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
       // O_t holds the products of the tiles before: S_t(j) was issued behind
       // them, and the next waits for this P.
       if (j >= 1 && __any_sync(0xffffffffu, m_new != m)) {
@@ -632,14 +642,33 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
           tmem_st32(taddr + colO + c * 32, o);
         }
       }
+      // P rounded to bf16, the type of V, for the product; l sums it unrounded.
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float pk[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const uint64_t y2 = f2_fma(f2_pack(sv[c][2 * x], sv[c][2 * x + 1]), sl2x2, negm2);
+          float e0, e1;
+          f2_unpack(y2, e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
+          pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
+        }
+        tmem_st16(taddr + colS + c * 16, pk);
+      }
+      float ps[8];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) f2_unpack(acc2[a], ps[2 * a], ps[2 * a + 1]);
+      l = l * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
       m = m_new;
-      if (dry) break;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[t]);
     }
     if (!ok) break;
-    if (!dry && !(ok = wait_all(&s_free[t], (seen - 1) & 1))) break;  // the last product
+    if (!(ok = wait_all(&s_free[t], (seen - 1) & 1))) break;  // the last product
     tc_fence_after();
     // What the combine pass has to know of the item: where its parts are.
     if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
@@ -668,15 +697,6 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
           for (int x = 0; x < 4; ++x) store_f32x8(dst + c * 32 + x * 8, o + x * 8);
         }
       }
-    }
-    if (dry) {
-      dry = false;
-      if (!begin()) return;
-      Walk x;
-      walk_start(p, tab, plan, x);
-      if (lane == 0) w = x;
-      __syncwarp();
-      continue;
     }
     tc_fence_before();
     mbar_arrive(&o_empty[t]);
@@ -713,13 +733,13 @@ struct Pages {
   }
 };
 
-// TMA loads of the shared part, one warp, from segment e on (work: there is
-// one, its page ids in `pages`). Per segment Q, then the tiles in the order the
-// products use them: `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1
-// for two row tiles, 2 for the two accumulators of one.
+// TMA loads of the shared part, one warp, from segment e on, its page ids in
+// `pages`. Per segment Q, then the tiles in the order the products use them:
+// `lead` K tiles, then V(i), K(i + lead) in turn; lead is 1 for two row tiles,
+// 2 for the two accumulators of one.
 __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                                           const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars, Walk& w,
-                                          Segment& e, bool work, Pages& pages, int lane) {
+                                          Segment& e, Pages& pages, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* q_full = bars.q_full();
   uint64_t* q_empty = bars.q_empty();
@@ -753,7 +773,7 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
     ++pos;
     return true;
   };
-  while (work) {
+  while (true) {
     if (!(ok = wait_all(q_empty, (kq & 1) ^ 1u))) break;
     if (lane == 0) {
       const uint32_t bytes = 128u * p.own.group * p.per_tile;
@@ -775,9 +795,8 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
         ok = ok && load(&tm_k, e.tile0 + i, k_id);
       }
     }
-    if (!ok) break;
-    work = walk_next(p, tab, w, e);
-    if (work) pages.start(p, e, lane);
+    if (!ok || !walk_next(p, tab, w, e)) break;
+    pages.start(p, e, lane);
   }
   if (!ok && lane == 0) {  // early exit: let the copies already issued land (bounded)
     for (uint32_t u = (pos > kStages ? pos - kStages : 0); u < pos; ++u)
@@ -787,9 +806,9 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
   __syncwarp();
 }
 
-// Products of the shared part, one warp; lane 0 issues.
+// Products of the shared part, one warp, from segment e on; lane 0 issues.
 __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars,
-                                             uint32_t tmem, Walk& w, Segment& e, bool work, int lane) {
+                                             uint32_t tmem, Walk& w, Segment& e, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* q_full = bars.q_full();
   uint64_t* q_empty = bars.q_empty();
@@ -821,11 +840,11 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
     __syncwarp();
   };
   auto issue_pv = [&](int t, bool first, uint32_t x) -> bool {
-    if (!wait_all(&p_full[t], cp[t] & 1)) return false;
     if (first) {  // O_t is overwritten: the previous segment's must have been read
       if (segs[t] > 0 && !wait_all(&o_empty[t], (segs[t] - 1) & 1)) return false;
       ++segs[t];
     }
+    if (!wait_all(&p_full[t], cp[t] & 1)) return false;
     tc_fence_after();
     if (lane == 0) {
       const uint64_t vd = desc_v(sKV + (x % kStages) * kTile);
@@ -839,49 +858,34 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
     ++cp[t];
     return true;
   };
-  auto release = [&](uint64_t* bar) {
-    if (lane == 0) umma_commit(bar);
+  auto release = [&](uint64_t* bar, bool now) {
+    if (lane == 0 && now) umma_commit(bar);
     __syncwarp();
   };
-  while (work) {
+  while (true) {
     if (!(ok = wait_all(q_full, kq & 1))) break;
     ++kq;
     const int n = e.tiles, lead = 2 - e.two;
-    for (int i = 0; ok && i < min(lead, n); ++i, ++pos) {
-      if (!(ok = wait_full(pos))) break;
-      if (e.two) {
-        issue_s(0, 0, pos);
-        issue_s(1, 1, pos);
-      } else {
-        issue_s(i, 0, pos);
-      }
-      release(&kv_empty[pos % kStages]);
-    }
-    if (!ok) break;
-    if (n <= lead) release(q_empty);
-    for (int i = 0; ok && i < n; ++i) {
-      const uint32_t vp = pos++;
+    // Products of V tile i and K tile i + lead, from the first K tiles on: both
+    // row tiles', or those of the accumulator whose turn it is.
+    for (int i = -lead; ok && i < n; ++i) {
       const bool more = i + lead < n;
-      const uint32_t kp = pos;
-      if (more) ++pos;
-      if (!(ok = wait_full(vp))) break;
+      const uint32_t vp = pos, kp = pos + (i >= 0 ? 1 : 0);
+      pos = kp + (more ? 1 : 0);
+      if (i >= 0 && !(ok = wait_full(vp))) break;
       if (more && !(ok = wait_full(kp))) break;
-      if (e.two) {
-        if (!(ok = issue_pv(0, i == 0, vp))) break;
-        if (more) issue_s(0, 0, kp);
-        if (!(ok = issue_pv(1, i == 0, vp))) break;
-        release(&kv_empty[vp % kStages]);
-        if (more) issue_s(1, 1, kp);
-      } else {
-        if (!(ok = issue_pv(i & 1, i < 2, vp))) break;
-        release(&kv_empty[vp % kStages]);
-        if (more) issue_s(i & 1, 0, kp);
+#pragma unroll 1
+      for (int x = 0; ok && x <= e.two; ++x) {
+        const int t = e.two ? x : (i + lead) & 1;
+        if (i >= 0) ok = issue_pv(t, i < lead, vp);
+        if (ok && more) issue_s(t, e.two ? t : 0, kp);
       }
-      if (more) release(&kv_empty[kp % kStages]);
-      if (more && i + 1 + lead == n) release(q_empty);  // the segment's last S
+      if (!ok) break;
+      release(&kv_empty[vp % kStages], i >= 0);
+      release(&kv_empty[kp % kStages], more);
+      release(q_empty, more && i + 1 + lead == n);  // the segment's last S
     }
-    if (!ok) break;
-    work = walk_next(p, tab, w, e);
+    if (!ok || !walk_next(p, tab, w, e)) break;
   }
   __syncwarp();
 }
@@ -920,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
 
   // Barriers and tensor memory: nothing that a kernel before this one writes.
-  if (warp == kWarpSetup && lane == 0) {
+  if (warp == kWarpSecond && lane == 0) {
     mbar_init(bars.q_full(), 1);
     mbar_init(bars.q_empty(), 1);
     for (int i = 0; i < kStages; ++i) {
@@ -944,7 +948,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(mg_empty, p.own.hkv);
     fence_barrier_init();
   }
-  if (warp == kWarpSetup) reinterpret_cast<uint32_t*>(smem + kOffZero)[lane] = 0u;
+  if (warp == kWarpSecond) reinterpret_cast<uint32_t*>(smem + kOffZero)[lane] = 0u;
   if (warp == kWarpProduct) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
@@ -968,69 +972,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (warp == kWarpPlan) {
-    if (!early) {
-      grid_dependency_wait();
-      in = read_inputs(p, lane);
-    }
-    for (int round = 0; round < 2; ++round) {
-      const Plan r = make_plan(p, tab, in, lane);
-      if (lane == 0) {
-        plan = r;
-        mbar_arrive(bars.planned());
-      }
-      grid_dependency_wait();
-      grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
-      if (round == 1) break;
-      bool same = true;
-      if (early) {
-        const Seen now = read_inputs(p, lane);
-        same = now.lo == in.lo && now.hi == in.hi && now.len == in.len;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) same &= now.raw[i] == in.raw[i];
-        same = __all_sync(0xffffffffu, same);
-        in = now;
-      }
-      if (lane == 0) {
-        *stale = !same;
-        mbar_arrive(bars.checked());
-      }
-      if (same) break;
-      named_sync(1, kThreads);  // everyone is done with the plan that was stale
-    }
-    if (blockIdx.x == 0) write_flags(p, tab, lane);
-    return;
-  }
-  if (warp == kWarpSetup) {  // no more work; takes part where everyone has to
-    if (wait_warp(p, bars.checked(), 0) && *stale) named_sync(1, kThreads);
-    return;
-  }
-  // The plan; `walk` goes by it, `look` reads by it from global memory before
-  // the check is back. All the warps that wait here do so a second time if the
-  // plan was stale.
-  auto begin = [&](auto walk, auto look) -> bool {
-    for (uint32_t round = 0;; ++round) {
-      if (!wait_warp(p, bars.planned(), round)) return false;
-      walk();
-      grid_dependency_wait();
-      look();
-      if (round == 1) return true;
-      if (!wait_warp(p, bars.checked(), 0)) return false;
-      if (!*stale) return true;
-      named_sync(1, kThreads);
-    }
-  };
 
+  // Round 0 with the plan; before anything is done by it, the check has to be
+  // back. If the plan was stale, round 1 with the new one.
+  // (A round through each warp's code before the plan was there, to fetch it
+  // into the instruction caches, made every size 3 to 35 % slower.)
   if (warp < 8) {
-    // Both parts' warps make the dry round; those of a CTA for the rows' own
-    // keys go on as consumers.
-    bool own = false;
-    softmax_warp(p, tab, plan, smem, bars, tmem, warp >> 2, warp, lane, [&]() -> bool {
-      if (!begin([] {}, [] {})) return false;
-      own = !plan.shared;
-      return !own;
-    });
-    if (own)
+    bool ok = false;
+    for (uint32_t round = 0; round < 2; ++round) {
+      if (!wait_warp(p, bars.planned(), round)) break;
+      grid_dependency_wait();
+      if (round == 0) {
+        if (!wait_warp(p, bars.checked(), 0)) break;
+        if (*stale) {
+          named_sync(1, kThreads);
+          continue;
+        }
+      }
+      ok = true;
+      break;
+    }
+    if (ok && plan.shared)
+      softmax_warp(p, tab, plan, smem, bars, tmem, warp >> 2, warp, lane);
+    else if (ok)
       decode::consume<kOwnStages, true>(p.own, smem + kCtrlBytes, full, empty,
                                         reinterpret_cast<const decode::StageDesc*>(smem + kOffDesc), smem + kOffZero,
                                         mg_full, mg_empty,
@@ -1039,56 +1003,103 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(bars.done());
-    return;
-  }
-  // Warps 8 and 9: products and loads of the shared part, or both loads of the
-  // rows' own keys.
-  decode::Windows<true> win;
-  Walk w;
-  Segment e{};
-  Pages pages;
-  bool work = false;
-  const bool ok = begin(
-      [&] {
-        if (plan.shared) {
-          walk_start(p, tab, plan, w);
-          work = walk_next(p, tab, w, e);
+  } else if (warp == kWarpProduct || warp == kWarpLoad) {
+    Walk w;
+    Segment e{};
+    Pages pages;
+    for (uint32_t round = 0; round < 2; ++round) {
+      if (!wait_warp(p, bars.planned(), round)) break;
+      bool work = plan.shared != 0;
+      if (work) {
+        walk_start(p, tab, plan, w);
+        work = walk_next(p, tab, w, e);
+      }
+      grid_dependency_wait();
+      if (work && warp == kWarpLoad) pages.start(p, e, lane);
+      if (round == 0) {
+        if (!wait_warp(p, bars.checked(), 0)) break;
+        if (*stale) {
+          named_sync(1, kThreads);
+          continue;
         }
-      },
-      [&] {
-        if (plan.shared) {
-          if (work && warp == kWarpLoad) pages.start(p, e, lane);
-        } else if (plan.u1 > plan.u0) {
-          win.tab = tab;
-          win.load_swin(p.own, lane, plan.at);
-          win.load_bwin(p.own, lane, plan.at,
-                        static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
+      }
+      if (work) {
+        if (warp == kWarpProduct)
+          product_warp(p, tab, smem, bars, tmem, w, e, lane);
+        else
+          load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, pages, lane);
+      }
+      break;
+    }
+    if (warp == kWarpProduct) {
+      // tensor memory is read by the eight warps until they are through
+      wait_warp(p, bars.done(), 0);
+      tc_fence_after();
+      tmem_dealloc(tmem, kTmemCols);
+    } else if (blockIdx.x == 0 && !plan.shared) {
+      write_flags(p, tab, lane);
+    }
+  } else {
+    const bool maker = warp == kWarpPlan;
+    decode::Windows<true> win;
+    win.tab = tab;
+    for (uint32_t round = 0; round < 2; ++round) {
+      if (maker) {
+        if (round == 0 && !early) grid_dependency_wait();
+        const Plan r = early ? make_plan(p, tab, in, lane) : make_large_plan(p, tab, lane);
+        if (lane == 0) {
+          plan = r;
+          mbar_arrive(bars.planned());
         }
-      });
-  if (ok) {
-    if (!plan.shared) {
-      if (plan.u1 > plan.u0)
+        __syncwarp();
+      } else if (!wait_warp(p, bars.planned(), round)) {
+        break;
+      }
+      grid_dependency_wait();
+      grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
+      if (maker && round == 0) {
+        bool same = true;
+        if (early) {
+          const Seen now = read_inputs(p, lane);
+          same = now.lo == in.lo && now.hi == in.hi && now.len == in.len;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) same &= now.raw[i] == in.raw[i];
+          same = __all_sync(0xffffffffu, same);
+          in = now;
+        }
+        if (lane == 0) {
+          *stale = !same;
+          mbar_arrive(bars.checked());
+        }
+        __syncwarp();
+      }
+      const bool work = !plan.shared && plan.u1 > plan.u0;
+      if (work) {
+        win.load_swin(p.own, lane, plan.at);
+        win.load_bwin(p.own, lane, plan.at,
+                      static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
+      }
+      if (round == 0) {
+        if (!wait_warp(p, bars.checked(), 0)) break;
+        if (*stale) {
+          named_sync(1, kThreads);
+          continue;
+        }
+      }
+      if (work)
         decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
                                           reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), win, plan.u0,
-                                          plan.u1 - plan.u0, plan.at, plan.before, plan.c, warp - decode::kCWarps, 2,
-                                          lane);
-    } else if (warp == kWarpLoad) {
-      load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, work, pages, lane);
-    } else {
-      product_warp(p, tab, smem, bars, tmem, w, e, work, lane);
+                                          plan.u1 - plan.u0, plan.at, plan.before, plan.c, maker ? 1 : 0, 2, lane);
+      break;
     }
-  }
-  if (warp == kWarpProduct) {
-    // tensor memory is read by the eight warps until they are through
-    wait_warp(p, bars.done(), 0);
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    if (!maker && blockIdx.x == 0 && plan.shared) write_flags(p, tab, lane);
   }
 }
 
 // ------------------------------------------------------------------ combine
-// A CTA per (row, query head); its four warps take every fourth run of 16 of
-// the row's parts and the first joins the warps' results. Lane l owns dims
+// kSplit: a CTA per (row, query head), whose four warps take every fourth run
+// of 16 of the row's parts, and the first joins the warps' results; where there
+// are enough rows and heads to fill the SMs, a warp for each. Lane l owns dims
 // 4l..4l+3. The row's parts are those of its group's item, one per CTA that
 // had a segment of it (two where the accumulators took alternate key tiles),
 // and those of its own keys. In a run the weights come from a maximum over
@@ -1113,15 +1124,19 @@ struct CombineParams {
   float* lse;
 };
 
+template <bool kSplit>
 __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const CombineParams p) {
   __shared__ float4 s_acc[kCombineWarps - 1][32];
   __shared__ float2 s_ml[kCombineWarps - 1];
-  const int b = blockIdx.x, hh = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
+  const int b = blockIdx.x, hh = kSplit ? blockIdx.y : blockIdx.y * kCombineWarps + (threadIdx.x >> 5);
+  const int warp = kSplit ? threadIdx.x >> 5 : 0;
+  constexpr int kWarps = kSplit ? kCombineWarps : 1;
   const int h = hh / p.group;
   const float NEG_INF = -__int_as_float(0x7f800000);
   grid_dependency_wait();
   grid_launch_dependents();
+  if (hh >= p.hq) return;
   const int flags = p.flags[b];
   const int2 rp = p.row_parts[b];
   const int4 it = p.items[static_cast<long long>(b) * p.hkv + h];
@@ -1134,7 +1149,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
   const int n = pn + own;
   float m = NEG_INF, l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int e0 = warp * kRun; e0 < n; e0 += kCombineWarps * kRun) {
+  for (int e0 = warp * kRun; e0 < n; e0 += kWarps * kRun) {
     const int x = e0 + (lane & (kRun - 1));
     int row = 0;
     if (x < pn)
@@ -1179,7 +1194,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
       }
     }
   }
-  if (n > kRun) {  // the other warps' results, in their order
+  if (kSplit && n > kRun) {  // the other warps' results, in their order
     if (warp > 0) {
       s_acc[warp - 1][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (lane == 0) s_ml[warp - 1] = make_float2(m, l);
@@ -1187,7 +1202,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Combi
     __syncthreads();
   }
   if (warp > 0) return;
-  for (int w = 1; w * kRun < n && w < kCombineWarps; ++w) {
+  for (int w = 1; w * kRun < n && w < kWarps; ++w) {
     const float2 ml = s_ml[w - 1];
     const float4 o = s_acc[w - 1][lane];
     if (ml.y == 0.f) continue;
@@ -1238,7 +1253,8 @@ int prefix_init(int device) {
   cudaError_t e = cudaFuncSetAttribute(prefix::shared_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        227 * 1024);
   cudaFuncAttributes a;
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, prefix::combine_kernel);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, prefix::combine_kernel<true>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, prefix::combine_kernel<false>);
   return cuda_status(e);
 }
 
@@ -1357,5 +1373,10 @@ extern "C" int la_paged_decode_shared_prefix(
   c.out_bs = out_batch_stride;
   c.out_hs = out_head_stride;
   c.lse = softmax_lse;
-  return cuda_status(launch_pdl(combine_kernel, dim3(batch, num_q_heads), dim3(32 * kCombineWarps), 0, stream, c));
+  // A row has about #SMs parts over the number of rows: one warp goes through
+  // them as fast as four once the rows and heads are four per SM.
+  const bool split = static_cast<int64_t>(batch) * num_q_heads < 4 * grid;
+  return cuda_status(launch_pdl(split ? combine_kernel<true> : combine_kernel<false>,
+                                dim3(batch, split ? num_q_heads : (num_q_heads + kCombineWarps - 1) / kCombineWarps),
+                                dim3(32 * kCombineWarps), 0, stream, c));
 }
