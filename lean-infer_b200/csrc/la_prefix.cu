@@ -90,14 +90,14 @@ static_assert(kOffWalk + 8 * kWalkBytes <= kOffTable && kOffTable + kMaxGroups *
 constexpr int kOwnStages = 2;
 constexpr int kWarpProduct = 8, kWarpLoad = 9, kWarpPlan = 10, kWarpSecond = 11;
 
-// The time model that divides the SMs (shared_ctas). Microseconds on a B200 at
-// ~1.9 GHz, fitted to the times of 15 calls with 2 to 146 CTAs for the shared
-// part; of those calls 13 get the division that measured fastest, or one within
-// 2 %, the others one within 11 %. A step with two row tiles (64 KB of K and V), with
-// one (128 KB); a unit (64 KB) of a row's own keys, without and with sub-chunks
-// to merge (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
-constexpr float kPairUs = 3.0f, kSingleUs = 3.6f, kUnitUs = 1.08f, kUnitMergedUs = 1.7f, kHbmUs = 0.0094f,
-                kSegmentUs = 4.0f;
+// The time model that divides the SMs (shared_ctas). Microseconds on a B200,
+// fitted to the times of 15 calls with 2 to 146 CTAs for the shared part: 12 of
+// them get the division that measured fastest or one within 3 %, the others one
+// within 12 %. A step with two row tiles (64 KB of K and V), with one (128 KB);
+// a unit (64 KB) of a row's own keys, without and with sub-chunks to merge
+// (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
+constexpr float kPairUs = 3.4f, kSingleUs = 3.8f, kUnitUs = 1.54f, kUnitMergedUs = 1.85f, kHbmUs = 0.0135f,
+                kSegmentUs = 4.8f;
 
 struct Params {
   decode::Params own;  // the rows' own keys; groups, tables, counts and scale of both parts
