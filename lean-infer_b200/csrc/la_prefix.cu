@@ -515,6 +515,12 @@ __device__ __forceinline__ int rows_of(const Params& p, const Segment& e, int t)
   return seqs * p.own.group;
 }
 
+// Lane 0's value, which the compiler knows to be the same in every lane.
+template <typename T>
+__device__ __forceinline__ T uniform(T x) {
+  return __shfl_sync(0xffffffffu, x, 0);
+}
+
 __device__ __forceinline__ uint64_t desc_kmajor(const uint8_t* tile) {
   return smem_desc_sw128(smem_u32(tile), 16, 1024);
 }
@@ -528,7 +534,7 @@ struct Bars {
   __device__ __forceinline__ uint64_t* kv_full() const { return b + 2; }   // [kStages]
   __device__ __forceinline__ uint64_t* kv_empty() const { return b + 6; }  // [kStages]
   __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2] S_t written
-  __device__ __forceinline__ uint64_t* s_free() const { return b + 12; }   // [2] P_t V done
+  __device__ __forceinline__ uint64_t* s_free() const { return b + 12; }   // [2] a segment's last P_t V done
   __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2] P_t written (128 arrivals)
   __device__ __forceinline__ uint64_t* o_empty() const { return b + 16; }  // [2] O_t stored (128)
   __device__ __forceinline__ uint64_t* planned() const { return b + 18; }  // the plan is in shared memory
@@ -568,7 +574,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
     __syncwarp();
     return more;
   };
-  uint32_t seen = 0;  // S tiles
+  uint32_t seen = 0, segs = 0;  // S tiles, segments
   bool ok = true;
   {
     Walk x;
@@ -668,7 +674,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       mbar_arrive(&p_full[t]);
     }
     if (!ok) break;
-    if (!(ok = wait_all(&s_free[t], (seen - 1) & 1))) break;  // the last product
+    if (!(ok = wait_all(&s_free[t], segs++ & 1))) break;  // the last product
     tc_fence_after();
     // What the combine pass has to know of the item: where its parts are.
     if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
@@ -806,9 +812,13 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
   __syncwarp();
 }
 
-// Products of the shared part, one warp, from segment e on; lane 0 issues.
+// Products of the shared part, one warp, from segment e on; one thread issues.
+// What the instructions take is the same in every lane and known to be so (from
+// lane 0's registers), and the issuing thread is chosen by elect.sync: issued
+// under `lane == 0`, from each lane's own registers, 128 rows behind 32768 shared
+// keys took 56.1 us, so 52.4.
 __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars,
-                                             uint32_t tmem, Walk& w, Segment& e, int lane) {
+                                             uint32_t tmem_base, Walk& w, Segment& e) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
   uint64_t* q_full = bars.q_full();
   uint64_t* q_empty = bars.q_empty();
@@ -818,18 +828,18 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
   uint64_t* s_free = bars.s_free();
   uint64_t* p_full = bars.p_full();
   uint64_t* o_empty = bars.o_empty();
-  uint8_t* sQ = smem + kOffQ;
-  uint8_t* sKV = smem + kOffKV;
+  const uint32_t tmem = uniform(tmem_base);
+  const uint64_t q_desc = uniform(desc_kmajor(smem + kOffQ)), k_desc = uniform(desc_kmajor(smem + kOffKV)),
+                 v_desc = uniform(desc_v(smem + kOffKV));
   // S_t over P_t is issued right behind the product that reads P_t: the
   // tensor core executes one thread's products in order.
-  int kq = 0;
-  uint32_t pos = 0;
-  uint32_t cp[2] = {0, 0}, segs[2] = {0, 0};
+  uint32_t kq = 0, pos = 0;
+  uint32_t p_par = 0, o_par = 3;  // bit t: parity of P_t's next phase, of O_t's
   bool ok = true;
   auto wait_full = [&](uint32_t x) -> bool { return wait_all(&kv_full[x % kStages], (x / kStages) & 1); };
   auto issue_s = [&](int t, int q, uint32_t x) {
-    if (lane == 0) {
-      const uint64_t ad = desc_kmajor(sQ + q * kTile), bd = desc_kmajor(sKV + (x % kStages) * kTile);
+    const uint64_t ad = q_desc + q * (kTile >> 4), bd = k_desc + (x % kStages) * (kTile >> 4);
+    if (elect_one()) {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         const int o = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
@@ -839,33 +849,33 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
     }
     __syncwarp();
   };
-  auto issue_pv = [&](int t, bool first, uint32_t x) -> bool {
+  auto issue_pv = [&](int t, bool first, bool last, uint32_t x) -> bool {
     if (first) {  // O_t is overwritten: the previous segment's must have been read
-      if (segs[t] > 0 && !wait_all(&o_empty[t], (segs[t] - 1) & 1)) return false;
-      ++segs[t];
+      if (!wait_all(&o_empty[t], (o_par >> t) & 1)) return false;
+      o_par ^= 1u << t;
     }
-    if (!wait_all(&p_full[t], cp[t] & 1)) return false;
+    if (!wait_all(&p_full[t], (p_par >> t) & 1)) return false;
+    p_par ^= 1u << t;
     tc_fence_after();
-    if (lane == 0) {
-      const uint64_t vd = desc_v(sKV + (x % kStages) * kTile);
+    const uint64_t vd = v_desc + (x % kStages) * (kTile >> 4);
+    if (elect_one()) {
 #pragma unroll
       for (int ks = 0; ks < kKeys / 16; ++ks)
         umma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + ks * 8, vd + ks * 128, kIdescPV,
                     (!first || ks > 0) ? 1u : 0u);
-      umma_commit(&s_free[t]);
+      if (last) umma_commit(&s_free[t]);
     }
     __syncwarp();
-    ++cp[t];
     return true;
   };
   auto release = [&](uint64_t* bar, bool now) {
-    if (lane == 0 && now) umma_commit(bar);
+    if (now && elect_one()) umma_commit(bar);
     __syncwarp();
   };
   while (true) {
     if (!(ok = wait_all(q_full, kq & 1))) break;
     ++kq;
-    const int n = e.tiles, lead = 2 - e.two;
+    const int n = uniform(e.tiles), two = uniform(e.two), lead = 2 - two;
     // Products of V tile i and K tile i + lead, from the first K tiles on: both
     // row tiles', or those of the accumulator whose turn it is.
     for (int i = -lead; ok && i < n; ++i) {
@@ -875,10 +885,10 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
       if (i >= 0 && !(ok = wait_full(vp))) break;
       if (more && !(ok = wait_full(kp))) break;
 #pragma unroll 1
-      for (int x = 0; ok && x <= e.two; ++x) {
-        const int t = e.two ? x : (i + lead) & 1;
-        if (i >= 0) ok = issue_pv(t, i < lead, vp);
-        if (ok && more) issue_s(t, e.two ? t : 0, kp);
+      for (int x = 0; ok && x <= two; ++x) {
+        const int t = two ? x : (i + lead) & 1;
+        if (i >= 0) ok = issue_pv(t, i < lead, !more, vp);
+        if (ok && more) issue_s(t, two ? t : 0, kp);
       }
       if (!ok) break;
       release(&kv_empty[vp % kStages], i >= 0);
@@ -1025,7 +1035,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (work) {
         if (warp == kWarpProduct)
-          product_warp(p, tab, smem, bars, tmem, w, e, lane);
+          product_warp(p, tab, smem, bars, tmem, w, e);
         else
           load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, pages, lane);
       }

@@ -272,6 +272,13 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
+// True in one lane of the warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // D (tmem) (+)= A (tmem) * B (smem descriptor), kind::f16, one CTA. A is
 // M x 16 in TMEM: row i in lane i, two 16-bit elements per 32-bit column
 // (the lower k index in the low half), 8 columns per instruction.
