@@ -53,17 +53,20 @@ namespace prefix {
 constexpr int kD = 128;
 constexpr int kRows = 128;             // query rows per tile
 constexpr int kKeys = 128;             // keys per K/V tile
+constexpr int kParts = 2;
+constexpr int kPart = kKeys / kParts;
 constexpr int kHalf = 128 * 128;       // 64 dims of 128 rows: 16 KB
 constexpr int kTile = 2 * kHalf;
 constexpr int kStages = 4;             // K/V tiles in flight
 constexpr int kThreads = 384;          // 12 warps: 168 registers for each thread
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColO = 256;        // O_t at kColO + 128 t; S_t at 128 t
-constexpr uint32_t kIdescQK = idesc_bf16_f32(128, kKeys, false, false);
+constexpr uint32_t kColO = 256;        // O_t at kColO + 128 t; S_t of a tile's first half at 128 t, of the second 64 behind
+constexpr uint32_t kIdescQK = idesc_bf16_f32(128, kPart, false, false);
 constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, false, true);
 // Shared memory. Control, both parts' barriers apart: they are initialised
 // before the CTA knows which part it takes. Then the part's data: Q0 Q1 and the
 // K/V ring; or the stages and the merge area of the decode warps.
+constexpr int kOffTmem = 224;
 constexpr int kOffOwnBar = 256;
 constexpr int kOffPlan = 384;
 constexpr int kOffStale = 448;
@@ -533,13 +536,14 @@ struct Bars {
   __device__ __forceinline__ uint64_t* q_empty() const { return b + 1; }   // its last S done
   __device__ __forceinline__ uint64_t* kv_full() const { return b + 2; }   // [kStages]
   __device__ __forceinline__ uint64_t* kv_empty() const { return b + 6; }  // [kStages]
-  __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2] S_t written
-  __device__ __forceinline__ uint64_t* s_free() const { return b + 12; }   // [2] a segment's last P_t V done
-  __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2] P_t written (128 arrivals)
-  __device__ __forceinline__ uint64_t* o_empty() const { return b + 16; }  // [2] O_t stored (128)
-  __device__ __forceinline__ uint64_t* planned() const { return b + 18; }  // the plan is in shared memory
-  __device__ __forceinline__ uint64_t* checked() const { return b + 19; }  // it was checked after the wait
-  __device__ __forceinline__ uint64_t* done() const { return b + 20; }     // a softmax warp is through (8)
+  __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2][2] S_t of each half written
+  __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2][2] P_t of each half written (128 arrivals)
+  __device__ __forceinline__ uint64_t* pv_done() const { return b + 18; }  // [2] P_t V done
+  __device__ __forceinline__ uint64_t* o_full() const { return b + 20; }   // [2] a segment's last P_t V done
+  __device__ __forceinline__ uint64_t* o_empty() const { return b + 22; }  // [2] O_t stored (128)
+  __device__ __forceinline__ uint64_t* planned() const { return b + 24; }  // the plan is in shared memory
+  __device__ __forceinline__ uint64_t* checked() const { return b + 25; }  // it was checked after the wait
+  __device__ __forceinline__ uint64_t* done() const { return b + 26; }     // a softmax warp is through (8)
 };
 
 __device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32_t parity) {
@@ -550,10 +554,11 @@ __device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32
 __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup* tab, const Plan& plan, uint8_t* smem,
                                              Bars bars, uint32_t tmem, int t, int warp, int lane) {
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
-  uint64_t* s_full = bars.s_full();
-  uint64_t* s_free = bars.s_free();
-  uint64_t* p_full = bars.p_full();
-  uint64_t* o_empty = bars.o_empty();
+  uint64_t* s_full = bars.s_full() + kParts * t;
+  uint64_t* p_full = bars.p_full() + kParts * t;
+  uint64_t* pv_done = bars.pv_done() + t;
+  uint64_t* o_full = bars.o_full() + t;
+  uint64_t* o_empty = bars.o_empty() + t;
   const float NEG_INF = -__int_as_float(0x7f800000);
   const int quarter = warp & 3;
   const int row = quarter * 32 + lane;
@@ -574,7 +579,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
     __syncwarp();
     return more;
   };
-  uint32_t seen = 0, segs = 0;  // S tiles, segments
+  uint32_t seen = 0, segs = 0;  // halves of key tiles, segments
   bool ok = true;
   {
     Walk x;
@@ -592,30 +597,33 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
     }
     const bool active = quarter * 32 < rows;  // rows of this warp
     float m = NEG_INF, l = 0.f;
-    for (int j = 0; j < n; ++j, ++seen) {
-      if (!(ok = wait_all(&s_full[t], seen & 1))) break;
+#pragma unroll 1
+    for (int j = 0; j < kParts * n; ++j, ++seen) {
+      const int half = j % kParts;
+      if (!(ok = wait_all(&s_full[half], (seen / kParts) & 1))) break;
       if (!active) {
-        mbar_arrive(&p_full[t]);
+        mbar_arrive(&p_full[half]);
         continue;
       }
       tc_fence_after();
-      float sv[4][32];
+      const uint32_t col = colS + half * kPart;
+      float sv[kPart / 32][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(taddr + colS + c * 32, sv[c]);
+      for (int c = 0; c < kPart / 32; ++c) tmem_ld32(taddr + col + c * 32, sv[c]);
       tc_wait_ld();
-      // keys of this tile, 128 but for the prefix's last
-      const int nvis = e.keys - (e.tile0 + (e.two ? j : 2 * j + t)) * kKeys;
+      // keys of this half, 64 but for the prefix's last tile
+      const int nvis = e.keys - (e.tile0 + (e.two ? j / kParts : 2 * (j / kParts) + t)) * kKeys - half * kPart;
       float mx[8];
 #pragma unroll
       for (int a = 0; a < 8; ++a) mx[a] = NEG_INF;
-      if (nvis >= kKeys) {
+      if (nvis >= kPart) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < kPart / 32; ++c)
 #pragma unroll
           for (int x = 0; x < 32; x += 2) mx[(x >> 1) & 7] = fmax3(mx[(x >> 1) & 7], sv[c][x], sv[c][x + 1]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < kPart / 32; ++c)
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
             const float x0 = (c * 32 + x < nvis) ? sv[c][x] : NEG_INF;
@@ -635,9 +643,14 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       uint64_t acc2[4];
 #pragma unroll
       for (int a = 0; a < 4; ++a) acc2[a] = 0ull;
-      // O_t holds the products of the tiles before: S_t(j) was issued behind
-      // them, and the next waits for this P.
+      // O_t is rescaled when it holds the products of the halves before; the
+      // next waits for this P. (The one but last is done, since S was issued
+      // behind it: the parity means the last.)
       if (j >= 1 && __any_sync(0xffffffffu, m_new != m)) {
+        if (kParts > 1) {
+          if (!(ok = wait_all(pv_done, (seen - 1) & 1))) break;
+          tc_fence_after();
+        }
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float o[32];
@@ -650,7 +663,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       }
       // P rounded to bf16, the type of V, for the product; l sums it unrounded.
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kPart / 32; ++c) {
         float pk[16];
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
@@ -662,7 +675,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
           acc2[x & 3] = f2_add(acc2[x & 3], f2_pack(e0, e1));
           pk[x] = __uint_as_float(pack_bf16x2(e0, e1));
         }
-        tmem_st16(taddr + colS + c * 16, pk);
+        tmem_st16(taddr + col + c * 16, pk);
       }
       float ps[8];
 #pragma unroll
@@ -671,10 +684,10 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       m = m_new;
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[t]);
+      mbar_arrive(&p_full[half]);
     }
     if (!ok) break;
-    if (!(ok = wait_all(&s_free[t], segs++ & 1))) break;  // the last product
+    if (!(ok = wait_all(o_full, segs++ & 1))) break;  // the last product
     tc_fence_after();
     // What the combine pass has to know of the item: where its parts are.
     if ((e.begin || e.end) && (e.two || t == 0) && row < rows && row % p.own.group == 0) {
@@ -705,7 +718,7 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       }
     }
     tc_fence_before();
-    mbar_arrive(&o_empty[t]);
+    mbar_arrive(o_empty);
   }
 }
 
@@ -812,6 +825,12 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
   __syncwarp();
 }
 
+// 1: a pair of row tiles, 0: the two accumulators of one.
+template <int kTwo>
+struct Pair {
+  static constexpr int value = kTwo;
+};
+
 // Products of the shared part, one warp, from segment e on; one thread issues.
 // What the instructions take is the same in every lane and known to be so (from
 // lane 0's registers), and the issuing thread is chosen by elect.sync: issued
@@ -819,84 +838,78 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tm_q, const CUtenso
 // keys took 56.1 us, so 52.4.
 __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars,
                                              uint32_t tmem_base, Walk& w, Segment& e) {
-  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
-  uint64_t* q_full = bars.q_full();
-  uint64_t* q_empty = bars.q_empty();
-  uint64_t* kv_full = bars.kv_full();
-  uint64_t* kv_empty = bars.kv_empty();
-  uint64_t* s_full = bars.s_full();
-  uint64_t* s_free = bars.s_free();
-  uint64_t* p_full = bars.p_full();
-  uint64_t* o_empty = bars.o_empty();
   const uint32_t tmem = uniform(tmem_base);
   const uint64_t q_desc = uniform(desc_kmajor(smem + kOffQ)), k_desc = uniform(desc_kmajor(smem + kOffKV)),
                  v_desc = uniform(desc_v(smem + kOffKV));
-  // S_t over P_t is issued right behind the product that reads P_t: the
-  // tensor core executes one thread's products in order.
   uint32_t kq = 0, pos = 0;
-  uint32_t p_par = 0, o_par = 3;  // bit t: parity of P_t's next phase, of O_t's
-  bool ok = true;
-  auto wait_full = [&](uint32_t x) -> bool { return wait_all(&kv_full[x % kStages], (x / kStages) & 1); };
-  auto issue_s = [&](int t, int q, uint32_t x) {
-    const uint64_t ad = q_desc + q * (kTile >> 4), bd = k_desc + (x % kStages) * (kTile >> 4);
-    if (elect_one()) {
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        const int o = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
-        umma_f16_ss(tmem + t * 128, ad + o, bd + o, kIdescQK, ks > 0 ? 1u : 0u);
+  uint32_t p_par = 0, o_par = 3;  // bit kParts t + part: parity of P_t's next phase; bit t: of O_t's
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
+  // S_t over P_t is issued right behind the product that reads P_t: the
+  // tensor core executes one thread's products in order. A step: the products of
+  // V tile i and K tile i + lead, both row tiles' or those of the accumulator
+  // whose turn it is.
+  auto segment = [&](auto pair) -> bool {
+    constexpr int kTwo = decltype(pair)::value, kLead = 2 - kTwo, kLast = (kParts << kTwo) - 1;
+    const int n = uniform(e.tiles);
+#pragma unroll 1
+    for (int i = -kLead; i < n; ++i) {
+      const bool pv = i >= 0, more = i + kLead < n;
+      const uint32_t vs = pos % kStages, v_par = (pos / kStages) & 1;
+      pos += pv;
+      const uint32_t ks = pos % kStages, k_par = (pos / kStages) & 1;
+      pos += more;
+      uint64_t *v_full = bars.kv_full() + vs, *k_full = bars.kv_full() + ks;
+      const bool here = (!pv || mbar_try_wait(v_full, v_par)) & (!more || mbar_try_wait(k_full, k_par));
+      if (!__all_sync(0xffffffffu, here)) {
+        if (pv && !wait(v_full, v_par)) return false;
+        if (more && !wait(k_full, k_par)) return false;
       }
-      umma_commit(&s_full[t]);
-    }
-    __syncwarp();
-  };
-  auto issue_pv = [&](int t, bool first, bool last, uint32_t x) -> bool {
-    if (first) {  // O_t is overwritten: the previous segment's must have been read
-      if (!wait_all(&o_empty[t], (o_par >> t) & 1)) return false;
-      o_par ^= 1u << t;
-    }
-    if (!wait_all(&p_full[t], (p_par >> t) & 1)) return false;
-    p_par ^= 1u << t;
-    tc_fence_after();
-    const uint64_t vd = v_desc + (x % kStages) * (kTile >> 4);
-    if (elect_one()) {
 #pragma unroll
-      for (int ks = 0; ks < kKeys / 16; ++ks)
-        umma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + ks * 8, vd + ks * 128, kIdescPV,
-                    (!first || ks > 0) ? 1u : 0u);
-      if (last) umma_commit(&s_free[t]);
+      for (int x = 0; x <= kLast; ++x) {
+        const int part = x >> kTwo, t = kTwo ? x & 1 : i & 1, b = kParts * t + part;
+        const bool first = i < kLead && part == 0;
+        const uint32_t col = tmem + t * 128 + part * kPart;
+        if (pv) {
+          if (first) {  // O_t is overwritten: the previous segment's must have been read
+            if (!wait(bars.o_empty() + t, (o_par >> t) & 1)) return false;
+            o_par ^= 1u << t;
+          }
+          if (!wait(bars.p_full() + b, (p_par >> b) & 1)) return false;
+          p_par ^= 1u << b;
+          tc_fence_after();
+        }
+        if (elect_one()) {
+          if (pv) {
+            const uint64_t vd = v_desc + vs * (kTile >> 4) + part * (kPart * 128 >> 4);
+#pragma unroll
+            for (int k = 0; k < kPart / 16; ++k)
+              umma_f16_ts(tmem + kColO + t * 128, col + k * 8, vd + k * 128, kIdescPV, (!first || k > 0) ? 1u : 0u);
+            if (kParts > 1) umma_commit(bars.pv_done() + t);
+            if (!more && part == kParts - 1) umma_commit(bars.o_full() + t);
+            if (x == kLast) umma_commit(bars.kv_empty() + vs);
+          }
+          if (more) {
+            const uint64_t qd = q_desc + kTwo * t * (kTile >> 4);
+            const uint64_t kd = k_desc + ks * (kTile >> 4) + part * (kPart * 128 >> 4);
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k) {
+              const int o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+              umma_f16_ss(col, qd + o, kd + o, kIdescQK, k > 0 ? 1u : 0u);
+            }
+            umma_commit(bars.s_full() + b);
+            if (x == kLast) umma_commit(bars.kv_empty() + ks);
+            if (x == kLast && i + 1 + kLead == n) umma_commit(bars.q_empty());  // the segment's last S
+          }
+        }
+        __syncwarp();
+      }
     }
-    __syncwarp();
     return true;
   };
-  auto release = [&](uint64_t* bar, bool now) {
-    if (now && elect_one()) umma_commit(bar);
-    __syncwarp();
-  };
-  while (true) {
-    if (!(ok = wait_all(q_full, kq & 1))) break;
-    ++kq;
-    const int n = uniform(e.tiles), two = uniform(e.two), lead = 2 - two;
-    // Products of V tile i and K tile i + lead, from the first K tiles on: both
-    // row tiles', or those of the accumulator whose turn it is.
-    for (int i = -lead; ok && i < n; ++i) {
-      const bool more = i + lead < n;
-      const uint32_t vp = pos, kp = pos + (i >= 0 ? 1 : 0);
-      pos = kp + (more ? 1 : 0);
-      if (i >= 0 && !(ok = wait_full(vp))) break;
-      if (more && !(ok = wait_full(kp))) break;
-#pragma unroll 1
-      for (int x = 0; ok && x <= two; ++x) {
-        const int t = two ? x : (i + lead) & 1;
-        if (i >= 0) ok = issue_pv(t, i < lead, !more, vp);
-        if (ok && more) issue_s(t, two ? t : 0, kp);
-      }
-      if (!ok) break;
-      release(&kv_empty[vp % kStages], i >= 0);
-      release(&kv_empty[kp % kStages], more);
-      release(q_empty, more && i + 1 + lead == n);  // the segment's last S
-    }
-    if (!ok || !walk_next(p, tab, w, e)) break;
-  }
+  do {
+    if (!wait(bars.q_full(), kq++ & 1)) break;
+    if (!(uniform(e.two) ? segment(Pair<1>{}) : segment(Pair<0>{}))) break;
+  } while (walk_next(p, tab, w, e));
   __syncwarp();
 }
 
@@ -923,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const Bars bars{reinterpret_cast<uint64_t*>(smem)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 192);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffTmem);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffOwnBar);
   uint64_t* empty = full + decode::kMaxStages;
   uint64_t* mg_full = empty + decode::kMaxStages;  // all consumer warps wrote their state
@@ -942,10 +955,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bars.kv_empty() + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars.s_full() + i, 1);
-      mbar_init(bars.s_free() + i, 1);
-      mbar_init(bars.p_full() + i, 128);
+      mbar_init(bars.pv_done() + i, 1);
+      mbar_init(bars.o_full() + i, 1);
       mbar_init(bars.o_empty() + i, 128);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bars.s_full() + i, 1);
+      mbar_init(bars.p_full() + i, 128);
     }
     mbar_init(bars.planned(), 1);
     mbar_init(bars.checked(), 1);
