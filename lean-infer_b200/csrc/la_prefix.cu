@@ -831,25 +831,29 @@ struct Pair {
   static constexpr int value = kTwo;
 };
 
-// Products of the shared part, one warp, from segment e on; one thread issues.
-// What the instructions take is the same in every lane and known to be so (from
-// lane 0's registers), and the issuing thread is chosen by elect.sync: issued
-// under `lane == 0`, from each lane's own registers, 128 rows behind 32768 shared
-// keys took 56.1 us, so 52.4.
+// Products of the shared part, from segment e on: a warp for each of the two
+// row tiles or accumulators, so that one warp's waits and arithmetic pass while
+// the other's products run (one warp for both: 128 rows behind 32768 shared keys
+// 52.5 us instead of 50). One thread issues. What the instructions take is the same
+// in every lane and known to be so (from lane 0's registers), and the issuing
+// thread is chosen by elect.sync (issued under `lane == 0`, from each lane's own
+// registers, they took 7 % longer).
 __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup* tab, uint8_t* smem, Bars bars,
-                                             uint32_t tmem_base, Walk& w, Segment& e) {
-  const uint32_t tmem = uniform(tmem_base);
+                                             uint32_t tmem_base, int tile, Walk& w, Segment& e, int lane) {
+  const int t = uniform(tile);
+  const uint32_t tmem = uniform(tmem_base), colS = tmem + t * 128, colO = tmem + kColO + t * 128;
   const uint64_t q_desc = uniform(desc_kmajor(smem + kOffQ)), k_desc = uniform(desc_kmajor(smem + kOffKV)),
                  v_desc = uniform(desc_v(smem + kOffKV));
-  uint32_t kq = 0, pos = 0;
-  uint32_t p_par = 0, o_par = 3;  // bit kParts t + part: parity of P_t's next phase; bit t: of O_t's
+  uint64_t *s_full = bars.s_full() + kParts * t, *p_full = bars.p_full() + kParts * t;
+  uint64_t *pv_done = bars.pv_done() + t, *o_full = bars.o_full() + t, *o_empty = bars.o_empty() + t;
+  uint32_t segs = 0, pos = 0, p_par = 0, o_par = 1;  // parities of the next phase
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(p, bar, parity); };
-  // S_t over P_t is issued right behind the product that reads P_t: the
-  // tensor core executes one thread's products in order. A step: the products of
-  // V tile i and K tile i + lead, both row tiles' or those of the accumulator
-  // whose turn it is.
+  // S over P is issued right behind the product that reads P: the tensor core
+  // executes one thread's products in order. A step: the products of V tile i
+  // and K tile i + lead; of a pair's tiles each warp takes all, of a single
+  // tile's those of its accumulator.
   auto segment = [&](auto pair) -> bool {
-    constexpr int kTwo = decltype(pair)::value, kLead = 2 - kTwo, kLast = (kParts << kTwo) - 1;
+    constexpr int kTwo = decltype(pair)::value, kLead = 2 - kTwo;
     const int n = uniform(e.tiles);
 #pragma unroll 1
     for (int i = -kLead; i < n; ++i) {
@@ -864,18 +868,19 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
         if (pv && !wait(v_full, v_par)) return false;
         if (more && !wait(k_full, k_par)) return false;
       }
+      // (the other warp's tiles are waited for as well: a parity tells one phase
+      // of a stage from the next, not from the one after)
+      if (!kTwo && (i & 1) != t) continue;
 #pragma unroll
-      for (int x = 0; x <= kLast; ++x) {
-        const int part = x >> kTwo, t = kTwo ? x & 1 : i & 1, b = kParts * t + part;
-        const bool first = i < kLead && part == 0;
-        const uint32_t col = tmem + t * 128 + part * kPart;
+      for (int part = 0; part < kParts; ++part) {
+        const bool first = i < kLead && part == 0, last = part == kParts - 1;
+        const uint32_t col = colS + part * kPart;
         if (pv) {
-          if (first) {  // O_t is overwritten: the previous segment's must have been read
-            if (!wait(bars.o_empty() + t, (o_par >> t) & 1)) return false;
-            o_par ^= 1u << t;
+          if (first) {  // O is overwritten: the previous segment's must have been read
+            if (!wait(o_empty, o_par)) return false;
+            o_par ^= 1;
           }
-          if (!wait(bars.p_full() + b, (p_par >> b) & 1)) return false;
-          p_par ^= 1u << b;
+          if (!wait(p_full + part, p_par)) return false;
           tc_fence_after();
         }
         if (elect_one()) {
@@ -883,10 +888,12 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
             const uint64_t vd = v_desc + vs * (kTile >> 4) + part * (kPart * 128 >> 4);
 #pragma unroll
             for (int k = 0; k < kPart / 16; ++k)
-              umma_f16_ts(tmem + kColO + t * 128, col + k * 8, vd + k * 128, kIdescPV, (!first || k > 0) ? 1u : 0u);
-            if (kParts > 1) umma_commit(bars.pv_done() + t);
-            if (!more && part == kParts - 1) umma_commit(bars.o_full() + t);
-            if (x == kLast) umma_commit(bars.kv_empty() + vs);
+              umma_f16_ts(colO, col + k * 8, vd + k * 128, kIdescPV, (!first || k > 0) ? 1u : 0u);
+            umma_commit(pv_done);
+            if (last) {
+              if (!more) umma_commit(o_full);
+              for (int c = kTwo; c < 2; ++c) umma_commit(bars.kv_empty() + vs);
+            }
           }
           if (more) {
             const uint64_t qd = q_desc + kTwo * t * (kTile >> 4);
@@ -896,18 +903,22 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
               const int o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
               umma_f16_ss(col, qd + o, kd + o, kIdescQK, k > 0 ? 1u : 0u);
             }
-            umma_commit(bars.s_full() + b);
-            if (x == kLast) umma_commit(bars.kv_empty() + ks);
-            if (x == kLast && i + 1 + kLead == n) umma_commit(bars.q_empty());  // the segment's last S
+            umma_commit(s_full + part);
+            if (last) {
+              for (int c = kTwo; c < 2; ++c) umma_commit(bars.kv_empty() + ks);
+              if (i + 2 * kLead >= n) umma_commit(bars.q_empty());  // this warp's last S of the segment
+            }
           }
         }
         __syncwarp();
       }
+      p_par ^= pv;
     }
+    if (!kTwo && t >= n && lane == 0) mbar_arrive(bars.q_empty());  // it had none
     return true;
   };
   do {
-    if (!wait(bars.q_full(), kq++ & 1)) break;
+    if (!wait(bars.q_full(), segs++ & 1)) break;
     if (!(uniform(e.two) ? segment(Pair<1>{}) : segment(Pair<0>{}))) break;
   } while (walk_next(p, tab, w, e));
   __syncwarp();
@@ -949,10 +960,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Barriers and tensor memory: nothing that a kernel before this one writes.
   if (warp == kWarpSecond && lane == 0) {
     mbar_init(bars.q_full(), 1);
-    mbar_init(bars.q_empty(), 1);
+    mbar_init(bars.q_empty(), 2);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bars.kv_full() + i, 1);
-      mbar_init(bars.kv_empty() + i, 1);
+      mbar_init(bars.kv_empty() + i, 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars.pv_done() + i, 1);
@@ -1029,44 +1040,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(bars.done());
-  } else if (warp == kWarpProduct || warp == kWarpLoad) {
+  } else {
+    const bool maker = warp == kWarpPlan;
     Walk w;
     Segment e{};
     Pages pages;
-    for (uint32_t round = 0; round < 2; ++round) {
-      if (!wait_warp(p, bars.planned(), round)) break;
-      bool work = plan.shared != 0;
-      if (work) {
-        walk_start(p, tab, plan, w);
-        work = walk_next(p, tab, w, e);
-      }
-      grid_dependency_wait();
-      if (work && warp == kWarpLoad) pages.start(p, e, lane);
-      if (round == 0) {
-        if (!wait_warp(p, bars.checked(), 0)) break;
-        if (*stale) {
-          named_sync(1, kThreads);
-          continue;
-        }
-      }
-      if (work) {
-        if (warp == kWarpProduct)
-          product_warp(p, tab, smem, bars, tmem, w, e);
-        else
-          load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, pages, lane);
-      }
-      break;
-    }
-    if (warp == kWarpProduct) {
-      // tensor memory is read by the eight warps until they are through
-      wait_warp(p, bars.done(), 0);
-      tc_fence_after();
-      tmem_dealloc(tmem, kTmemCols);
-    } else if (blockIdx.x == 0 && !plan.shared) {
-      write_flags(p, tab, lane);
-    }
-  } else {
-    const bool maker = warp == kWarpPlan;
     decode::Windows<true> win;
     win.tab = tab;
     for (uint32_t round = 0; round < 2; ++round) {
@@ -1081,8 +1059,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else if (!wait_warp(p, bars.planned(), round)) {
         break;
       }
+      bool work = plan.shared ? !maker : plan.u1 > plan.u0 && warp >= kWarpPlan;
+      if (work && plan.shared) {
+        walk_start(p, tab, plan, w);
+        work = walk_next(p, tab, w, e);
+      }
       grid_dependency_wait();
-      grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
+      if (warp >= kWarpPlan) grid_launch_dependents();  // the combine pass waits for this grid's end before it reads
       if (maker && round == 0) {
         bool same = true;
         if (early) {
@@ -1099,11 +1082,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      const bool work = !plan.shared && plan.u1 > plan.u0;
-      if (work) {
+      if (work && !plan.shared) {
         win.load_swin(p.own, lane, plan.at);
         win.load_bwin(p.own, lane, plan.at,
                       static_cast<int>((plan.u0 - plan.before) * p.own.tc / p.own.block_size));
+      } else if (work && warp == kWarpLoad) {
+        pages.start(p, e, lane);
       }
       if (round == 0) {
         if (!wait_warp(p, bars.checked(), 0)) break;
@@ -1112,13 +1096,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
       }
-      if (work)
-        decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
-                                          reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), win, plan.u0,
-                                          plan.u1 - plan.u0, plan.at, plan.before, plan.c, maker ? 1 : 0, 2, lane);
+      if (work) {
+        if (!plan.shared)
+          decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
+                                            reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), win, plan.u0,
+                                            plan.u1 - plan.u0, plan.at, plan.before, plan.c, maker ? 1 : 0, 2, lane);
+        else if (warp == kWarpLoad)
+          load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, pages, lane);
+        else
+          product_warp(p, tab, smem, bars, tmem, warp == kWarpSecond, w, e, lane);
+      }
       break;
     }
-    if (!maker && blockIdx.x == 0 && plan.shared) write_flags(p, tab, lane);
+    if (warp == kWarpProduct) {
+      // tensor memory is read by the eight warps until they are through
+      wait_warp(p, bars.done(), 0);
+      tc_fence_after();
+      tmem_dealloc(tmem, kTmemCols);
+    } else if (blockIdx.x == 0 && warp == (plan.shared ? kWarpPlan : kWarpLoad)) {
+      write_flags(p, tab, lane);
+    }
   }
 }
 
