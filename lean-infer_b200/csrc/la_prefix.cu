@@ -94,13 +94,12 @@ constexpr int kOwnStages = 2;
 constexpr int kWarpProduct = 8, kWarpLoad = 9, kWarpPlan = 10, kWarpSecond = 11;
 
 // The time model that divides the SMs (shared_ctas). Microseconds on a B200,
-// fitted to the times of 15 calls with 2 to 146 CTAs for the shared part: 12 of
-// them get the division that measured fastest or one within 3 %, the others one
-// within 12 %. A step with two row tiles (64 KB of K and V), with one (128 KB);
+// fitted to the times of 15 calls with 2 to 146 CTAs for the shared part: all get
+// the division that measured fastest or one within 3.5 %. A step with two row tiles (64 KB of K and V), with one (128 KB);
 // a unit (64 KB) of a row's own keys, without and with sub-chunks to merge
 // (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
-constexpr float kPairUs = 3.4f, kSingleUs = 3.8f, kUnitUs = 1.54f, kUnitMergedUs = 1.85f, kHbmUs = 0.0135f,
-                kSegmentUs = 4.8f;
+constexpr float kPairUs = 1.45f, kSingleUs = 2.2f, kUnitUs = 1.25f, kUnitMergedUs = 1.45f, kHbmUs = 0.0112f,
+                kSegmentUs = 4.f;
 
 struct Params {
   decode::Params own;  // the rows' own keys; groups, tables, counts and scale of both parts
@@ -277,17 +276,17 @@ __device__ __forceinline__ int shared_ctas(const Params& p, float pair_steps, fl
     const float x = static_cast<float>(P), cs = fminf(x, steps), co = fminf(static_cast<float>(grid - P), units);
     const float f = fmaxf(1.f, cs * loads + co * own_loads);
     // whole items per CTA or CTAs per item: P * per_item is whole up to rounding
-    const float y = x * per_item, odd = fabsf(y - rintf(y)) > 1e-3f ? kSegmentUs : 0.f;
+    const float y = x * per_item, odd = x < steps && fabsf(y - rintf(y)) > 1e-3f ? kSegmentUs : 0.f;
     const float t = fmaxf(__fdividef(a * f * f * f + b * sqrtf(f), cs) + odd,
                           units > 0.f ? __fdividef(own_work, fmaxf(co, 1e-6f)) : 0.f);
-    if (t < best) {
+    if (t <= best) {
       best = t;
       at = P;
     }
   }
   // positive floats compare as their bits do
   const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(best));
-  return static_cast<int>(__reduce_min_sync(0xffffffffu, __float_as_uint(best) == least ? at : 0x7fffffffu));
+  return static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(best) == least ? at : 0));
 }
 
 // The part that the CTA takes, and its number there. Neighbouring CTAs mostly
