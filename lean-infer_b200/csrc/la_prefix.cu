@@ -95,7 +95,8 @@ constexpr int kWarpProduct = 8, kWarpLoad = 9, kWarpPlan = 10, kWarpSecond = 11;
 
 // The time model that divides the SMs (shared_ctas). Microseconds on a B200,
 // fitted to the times of 15 calls with 2 to 146 CTAs for the shared part: all get
-// the division that measured fastest or one within 3.5 %. A step with two row tiles (64 KB of K and V), with one (128 KB);
+// the division that measured fastest or one within 3.5 %
+// (with fractional steps per CTA, 9 %). A step with two row tiles (64 KB of K and V), with one (128 KB);
 // a unit (64 KB) of a row's own keys, without and with sub-chunks to merge
 // (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
 constexpr float kPairUs = 1.45f, kSingleUs = 2.2f, kUnitUs = 1.25f, kUnitMergedUs = 1.45f, kHbmUs = 0.0112f,
@@ -258,14 +259,18 @@ __device__ __forceinline__ int part_start(int c, int T, int G, float inv_G) {
 
 // CTAs of the shared part, an even number, from its steps, the rows' units and
 // the items: the one of least time by a model, 64 numbers of CTAs tried at
-// once. Both parts take the time of their work over their CTAs; where all CTAs
-// together would load more than HBM gives, by a factor f, the steps with two
-// row tiles, whose loads are needed soonest, take f^3 as long, the others,
-// whose loads are twice as many, f^0.5. A CTA whose range is not within one
-// item has two segments to store.
+// once, of several the one with most, whose busy CTAs are the closest (8 rows
+// 12 us instead of 12.7). The shared part takes the time of a CTA's steps, the
+// other that of its units over its CTAs; where all CTAs together would load more
+// than HBM gives, by a factor f, the steps with two row tiles, whose loads are
+// needed soonest, take f^3 as long, the others, whose loads are twice as many,
+// f^0.5. A CTA whose range is not within one item has two segments to store.
+// Where there is a CTA for every step and unit, the model has nothing to weigh.
 __device__ __forceinline__ int shared_ctas(const Params& p, float pair_steps, float single_steps, float units,
                                            int items, int grid, int lane) {
-  const float a = pair_steps * kPairUs, b = single_steps * kSingleUs, steps = pair_steps + single_steps;
+  const float steps = pair_steps + single_steps, avg = __fdividef(1.f, steps);
+  if (steps + units < static_cast<float>(grid)) return (grid - static_cast<int>(units)) & ~1;
+  const float a = pair_steps * kPairUs, b = single_steps * kSingleUs;
   const float unit = p.own.nsub > 1 ? kUnitMergedUs : kUnitUs, own_work = units * unit;
   const float loads = __fdividef(pair_steps + 2.f * single_steps, a + b) * kHbmUs;  // of one CTA, of HBM's rate
   const float own_loads = __fdividef(kHbmUs, unit), per_item = __fdividef(1.f, static_cast<float>(items));
@@ -277,7 +282,7 @@ __device__ __forceinline__ int shared_ctas(const Params& p, float pair_steps, fl
     const float f = fmaxf(1.f, cs * loads + co * own_loads);
     // whole items per CTA or CTAs per item: P * per_item is whole up to rounding
     const float y = x * per_item, odd = x < steps && fabsf(y - rintf(y)) > 1e-3f ? kSegmentUs : 0.f;
-    const float t = fmaxf(__fdividef(a * f * f * f + b * sqrtf(f), cs) + odd,
+    const float t = fmaxf((a * f * f * f + b * sqrtf(f)) * avg * ceilf(__fdividef(steps, cs) - 1e-3f) + odd,
                           units > 0.f ? __fdividef(own_work, fmaxf(co, 1e-6f)) : 0.f);
     if (t <= best) {
       best = t;
