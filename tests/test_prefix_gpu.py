@@ -110,6 +110,16 @@ CASES = {
     "one_kv_head": ([(251, 2048), (5, 256)], own(260, 1, 300), 256, 2, 1),
     "many_rows": ([(600, 512), (500, 256)], own(1105, 0, 30), 256, 4, 2),
     "many_small_groups": ([(2, 64 * (1 + i % 5)) for i in range(150)], own(303, 0, 20), 64, 2, 1),
+    "rows_256_groups_32": ([(8, 64 * (i % 4)) for i in range(32)], own(256, 0, 90), 64, 8, 4),
+    "rows_257_groups_32": ([(8, 64 * (i % 4)) for i in range(32)], own(257, 0, 90), 64, 8, 4),
+    "rows_256_groups_33": ([(7, 64 * (i % 4)) for i in range(33)], own(256, 0, 90), 64, 8, 4),
+    "six_hundred_groups": ([(2, 32 * (i % 7)) for i in range(600)], own(1205, 0, 40), 32, 2, 1),
+    "groups_of_nothing": ([(0, 64)] * 300 + [(5, 192)] + [(0, 0)] * 300 + [(1, 64), (30, 64)], own(40, 0, 50), 64, 16, 8),
+    "halves_of_key_tiles": ([(4, 16), (4, 64), (4, 80), (4, 128), (4, 144), (40, 192), (4, 208), (4, 336)],
+                            own(68, 0, 20), 16, 16, 8),
+    "group_8_one_head": ([(33, 1000), (2, 512)], own(35, 0, 200), 16, 8, 1),
+    "no_own_keys": ([(100, 4096)], [0] * 100, 256, 16, 8),
+    "mostly_own_keys": ([(2, 16)], own(100, 500, 900), 16, 16, 8),
     "long": ([(40, 20000)], own(40, 1, 700), 256, 16, 8),
     "long_for_two": ([(2, 30011), (3, 17)], own(5, 1, 9000), 16, 16, 8),
 }
@@ -167,6 +177,67 @@ def test_large_scores(pkg, cuda_dev):
     e = 2 * 136 * 2.0 ** -24 * abss[:, None, :, None]
     assert bool(((out.double() - ref).abs() <= (2.0 ** -8 + e) * (absv + ref.abs()) + 2.0 ** -12 * absv).all())
     assert bool(((lse[:, :, 0].double() - rlse).abs() <= abss * 136 * 2.0 ** -24 + 2.0 ** -18 * (1 + rlse.abs())).all())
+
+
+def test_rising_scores(pkg, cuda_dev):
+    """Each 64 keys' scores exceed those before by ten and more powers of two, so
+    that what has been summed is scaled down again and again; and the same keys
+    in falling order."""
+    for fall in (False, True):
+        w = Batch(cuda_dev, [(40, 1536), (5, 1100)], [0] * 45, 256, 16, 8, seed=17)
+        w.q.abs_()
+        w.k.abs_()
+        n = w.lens[0].item()
+        ramp = torch.arange(n, device=cuda_dev) / 64
+        for row in (0, 40):
+            pages = w.table[row, :-(-w.lens[row].item() // 256)].long()
+            for j, page in enumerate(pages.flip(0) if fall else pages):
+                r = ramp[256 * j:256 * j + 256]
+                w.k[page] *= (r.flip(0) if fall else r)[:, None, None].to(torch.bfloat16)
+        out, lse = w.call(pkg)
+        pkg.check_device_errors(cuda_dev.index)
+        ref, rlse, absv, abss = opa.paged_decode_f64(w.q, w.k, w.v, w.table, w.lens)
+        e = 2 * 136 * 2.0 ** -24 * abss[:, None, :, None]  # as in test_large_scores
+        assert bool(((out.double() - ref).abs() <= (2.0 ** -8 + e) * (absv + ref.abs()) + 2.0 ** -12 * absv).all())
+        assert bool(((lse[:, :, 0].double() - rlse).abs() <= abss * 136 * 2.0 ** -24 + 2.0 ** -18 * (1 + rlse.abs())).all())
+
+
+def test_lengths_and_groups_written_by_the_kernel_in_front(pkg, cuda_dev):
+    """The call starts beside the end of the kernel before it. That one writes the
+    lengths and groups here (as bits, into pages of their own), so that what the
+    call saw first is out of date."""
+    a = Batch(cuda_dev, [(10, 640), (4, 128), (0, 0), (9, 64)], own(24, 0, 200, 1), 64, 16, 8, seed=18)
+    b = Batch(cuda_dev, [(0, 0), (20, 320), (1, 64), (3, 64)], own(24, 0, 500, 2), 64, 16, 8, seed=19)
+    nb, tokens = 64, 64 * 64
+    pages = [torch.zeros(nb, 64, 8, 128, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2)]
+    at = pages[0].view(torch.int32)[nb - 1, 63]
+    table, pos = torch.arange(nb, dtype=torch.int32, device=cuda_dev)[None], torch.zeros(1, dtype=torch.int64, device=cuda_dev)
+    news = []
+    for w in (a, b):
+        new = torch.zeros(1, tokens, 8, 128, dtype=torch.bfloat16, device=cuda_dev)
+        bits = new.view(torch.int32)[0, -1]
+        bits[0, :24], bits[1, :4], bits[2, :5] = w.lens, w.prefix, w.cu
+        news.append(new)
+
+    def both():
+        got = []
+        for w, new in zip((a, b), news):
+            pkg.paged_kv_write(new, new, pos, table, *pages)
+            got.append(pkg.flash_attn_with_shared_prefix(w.q, w.k, w.v, at[0, :24], w.table, at[1, :4], at[2, :5],
+                                                         return_softmax_lse=True))
+        return got
+
+    for _ in range(10):
+        for w, got in zip((a, b), both()):
+            w.check(pkg, got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [both() for _ in range(4)]
+    for _ in range(3):
+        graph.replay()
+        for x in got:
+            a.check(pkg, x[0])
+            b.check(pkg, x[1])
 
 
 def test_same_as_plain_decode(pkg, cuda_dev):
