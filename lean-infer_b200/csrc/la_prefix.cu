@@ -537,9 +537,9 @@ __device__ __forceinline__ uint64_t desc_v(const uint8_t* tile) { return smem_de
 struct Bars {
   uint64_t* b;
   __device__ __forceinline__ uint64_t* q_full() const { return b + 0; }    // a segment's Q landed
-  __device__ __forceinline__ uint64_t* q_empty() const { return b + 1; }   // its last S done
+  __device__ __forceinline__ uint64_t* q_empty() const { return b + 1; }   // both product warps' last S done
   __device__ __forceinline__ uint64_t* kv_full() const { return b + 2; }   // [kStages]
-  __device__ __forceinline__ uint64_t* kv_empty() const { return b + 6; }  // [kStages]
+  __device__ __forceinline__ uint64_t* kv_empty() const { return b + 6; }  // [kStages] both product warps are through
   __device__ __forceinline__ uint64_t* s_full() const { return b + 10; }   // [2][2] S_t of each half written
   __device__ __forceinline__ uint64_t* p_full() const { return b + 14; }   // [2][2] P_t of each half written (128 arrivals)
   __device__ __forceinline__ uint64_t* pv_done() const { return b + 18; }  // [2] P_t V done
@@ -872,9 +872,16 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
         if (pv && !wait(v_full, v_par)) return false;
         if (more && !wait(k_full, k_par)) return false;
       }
-      // (the other warp's tiles are waited for as well: a parity tells one phase
-      // of a stage from the next, not from the one after)
-      if (!kTwo && (i & 1) != t) continue;
+      // A parity tells one phase of a stage from the next, not from the one after:
+      // the other warp's tiles are waited for as well, and released by both.
+      if (!kTwo && (i & 1) != t) {
+        if (lane == 0) {
+          if (pv) mbar_arrive(bars.kv_empty() + vs);
+          if (more) mbar_arrive(bars.kv_empty() + ks);
+        }
+        __syncwarp();
+        continue;
+      }
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
         const bool first = i < kLead && part == 0, last = part == kParts - 1;
@@ -896,7 +903,7 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
             umma_commit(pv_done);
             if (last) {
               if (!more) umma_commit(o_full);
-              for (int c = kTwo; c < 2; ++c) umma_commit(bars.kv_empty() + vs);
+              umma_commit(bars.kv_empty() + vs);
             }
           }
           if (more) {
@@ -909,7 +916,7 @@ __device__ __forceinline__ void product_warp(const Params& p, const PrefixGroup*
             }
             umma_commit(s_full + part);
             if (last) {
-              for (int c = kTwo; c < 2; ++c) umma_commit(bars.kv_empty() + ks);
+              umma_commit(bars.kv_empty() + ks);
               if (i + 2 * kLead >= n) umma_commit(bars.q_empty());  // this warp's last S of the segment
             }
           }

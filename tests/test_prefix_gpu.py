@@ -120,6 +120,8 @@ CASES = {
     "group_8_one_head": ([(33, 1000), (2, 512)], own(35, 0, 200), 16, 8, 1),
     "no_own_keys": ([(100, 4096)], [0] * 100, 256, 16, 8),
     "mostly_own_keys": ([(2, 16)], own(100, 500, 900), 16, 16, 8),
+    "many_segments_per_cta": ([(3 + i * 5 % 11, 64 * (1 + i * 7 % 9)) for i in range(24)], own(190, 1500, 2500), 64, 16, 8),
+    "pairs_and_singles_in_turn": ([(20 + i * 37 % 190, 128 * (1 + i % 5)) for i in range(9)], own(1030, 60, 200), 128, 8, 4),
     "long": ([(40, 20000)], own(40, 1, 700), 256, 16, 8),
     "long_for_two": ([(2, 30011), (3, 17)], own(5, 1, 9000), 16, 16, 8),
 }
