@@ -177,6 +177,15 @@ struct Windows {
   }
 };
 
+// Stage of unit k, and the parity of its phase. kStages 0: two or three, as
+// `stages` says.
+template <int kStages>
+__device__ __forceinline__ int stage_of(int k, int stages, uint32_t& ph) {
+  const int n = kStages > 0 ? k / kStages : stages == 2 ? k / 2 : k / 3;
+  ph = static_cast<uint32_t>(n & 1);
+  return k - n * (kStages > 0 ? kStages : stages);
+}
+
 // A producer warp: units u0 .. u0 + n_units - 1 of the line, from sequence b0
 // (whose first unit is pb0) on, pid-th of nprod producers.
 template <int kStages, bool kPrefix>
@@ -184,7 +193,7 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
                                         const CUtensorMap& tm_k1, const CUtensorMap& tm_v1, const Params& p,
                                         uint8_t* smem, uint64_t* full, uint64_t* empty, StageDesc* descs,
                                         Windows<kPrefix>& w, long long u0, long long n_units, int b0, long long pb0,
-                                        int cta, int pid, int nprod, int lane) {
+                                        int cta, int pid, int nprod, int lane, int stages = kStages) {
   const int hkv = p.hkv;
   // kPrefix: a row's own keys are read once, and beside them run CTAs that
   // read the shared ones, and code, from L2.
@@ -246,8 +255,8 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
         nbwin = w.ids(p, lane, nbb, 0);
       }
     }
-    const int s = k % kStages;
-    const uint32_t ph = static_cast<uint32_t>((k / kStages) & 1);
+    uint32_t ph;
+    const int s = stage_of<kStages>(k, stages, ph);
     if (!mbar_wait(&empty[s], ph ^ 1u, p.err, LA_DEVERR_WAIT_TIMEOUT)) break;
     uint8_t* st = smem + s * p.stage_bytes;
 
@@ -356,8 +365,11 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
   // On an early exit, let the copies this warp issued land before the CTA
   // releases its shared memory (bounded).
   if (k < nu) {
-    for (int kk = (k > kStages ? k - kStages : 0); kk < k; ++kk)
-      if (kk % nprod == pid) mbar_wait(&full[kk % kStages], static_cast<uint32_t>((kk / kStages) & 1), nullptr, 0);
+    for (int kk = (k > stages ? k - stages : 0); kk < k; ++kk) {
+      uint32_t ph;
+      const int s = stage_of<kStages>(kk, stages, ph);
+      if (kk % nprod == pid) mbar_wait(&full[s], ph, nullptr, 0);
+    }
   }
 }
 
@@ -365,7 +377,8 @@ __device__ __forceinline__ void produce(const CUtensorMap& tm_q, const CUtensorM
 template <int kStages, bool kPrefix>
 __device__ __forceinline__ void consume(const Params& p, uint8_t* smem, uint64_t* full, uint64_t* empty,
                                         const StageDesc* descs, const uint8_t* zero_row, uint64_t* mg_full,
-                                        uint64_t* mg_empty, float* merge, long long n_units, int warp, int lane) {
+                                        uint64_t* mg_empty, float* merge, long long n_units, int warp, int lane,
+                                        int stages = kStages) {
   const int hkv = p.hkv;
   const int w = warp;
   const int j = w / hkv;
@@ -383,8 +396,8 @@ __device__ __forceinline__ void consume(const Params& p, uint8_t* smem, uint64_t
 
   const int nu = static_cast<int>(n_units);
   for (int k = 0; k < nu; ++k) {
-    const int s = k % kStages;
-    const uint32_t ph = static_cast<uint32_t>((k / kStages) & 1);
+    uint32_t ph;
+    const int s = stage_of<kStages>(k, stages, ph);
     if (!mbar_wait(&full[s], ph, p.err, LA_DEVERR_WAIT_TIMEOUT)) return;
     const StageDesc d = descs[s];
     uint8_t* st = smem + s * p.stage_bytes;

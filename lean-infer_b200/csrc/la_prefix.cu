@@ -83,27 +83,25 @@ constexpr size_t kSmemBytes = kOffKV + kStages * kTile + 1024;  // + alignment t
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(kOffWalk + 8 * kWalkBytes <= kOffTable && kOffTable + kMaxGroups * sizeof(PrefixGroup) <= kCtrlBytes,
               "control area");
-// Warps behind the eight of softmax or consumers: two of the shared part, two
-// that load the rows' own keys, the first of which makes the plan.
-// Pipeline stages (of 64 KB) of the decode warps. What they keep in flight,
-// 128 KB on each SM, draws all that HBM has; the third stage that fits only
-// makes every load wait longer, and the shared part, whose CTAs keep less in
-// flight, waits with them (128 rows behind 2048 keys: 74 us with three, 61
-// with two).
-constexpr int kOwnStages = 2;
+// Warps behind the eight of softmax or consumers. Shared part: the products of
+// tile 0 and (kWarpSecond) 1, and the loads between them. Own keys: the last two
+// load. kWarpPlan makes the plan.
 constexpr int kWarpProduct = 8, kWarpLoad = 9, kWarpPlan = 10, kWarpSecond = 11;
 
 // The time model that divides the SMs (shared_ctas). Microseconds on a B200,
 // fitted to the times of 15 calls with 2 to 146 CTAs for the shared part: all get
-// the division that measured fastest or one within 3.5 %
+// the division that measured fastest or one within 4 %
 // (with fractional steps per CTA, 9 %). A step with two row tiles (64 KB of K and V), with one (128 KB);
 // a unit (64 KB) of a row's own keys, without and with sub-chunks to merge
 // (nsub > 1); 64 KB at the rate of HBM; a second segment of a CTA.
-constexpr float kPairUs = 1.45f, kSingleUs = 2.2f, kUnitUs = 1.25f, kUnitMergedUs = 1.45f, kHbmUs = 0.0112f,
-                kSegmentUs = 4.f;
+constexpr float kPairUs = 1.16f, kSingleUs = 2.14f, kUnitUs = 0.964f, kUnitMergedUs = 1.236f, kHbmUs = 0.0094f,
+                kSegmentUs = 4.5f;
 
 struct Params {
   decode::Params own;  // the rows' own keys; groups, tables, counts and scale of both parts
+  // Of 64 KB, of the decode warps: three, or two where three do not fit (128 rows
+  // behind 2048 keys, mostly their own: 50.2 us with three, 53.2 with two).
+  int stages;
   int box_keys;        // keys per TMA box, a power of two that divides the block size
   int per_tile;        // sequences per row tile: 128 / group
   uint32_t tile_magic; // ceil(2^32 / per_tile): x / per_tile is the high word of x * magic for x < 2^25
@@ -512,6 +510,7 @@ __device__ __forceinline__ bool walk_next(const Params& p, const PrefixGroup* ta
   return true;
 }
 
+static_assert(kOffDesc + 3 * sizeof(decode::StageDesc) <= kOffZero, "a descriptor per stage");
 static_assert(sizeof(Walk) <= 64 && sizeof(Segment) + 64 <= kWalkBytes, "a softmax warp's walk");
 
 // Key tiles that tile t's accumulator takes, and the i-th of them.
@@ -988,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bars.planned(), 1);
     mbar_init(bars.checked(), 1);
     mbar_init(bars.done(), 8);
-    for (int s = 0; s < kOwnStages; ++s) {
+    for (int s = 0; s < 3; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], decode::kCWarps);
     }
@@ -1043,11 +1042,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && plan.shared)
       softmax_warp(p, tab, plan, smem, bars, tmem, warp >> 2, warp, lane);
     else if (ok)
-      decode::consume<kOwnStages, true>(p.own, smem + kCtrlBytes, full, empty,
+      decode::consume<0, true>(p.own, smem + kCtrlBytes, full, empty,
                                         reinterpret_cast<const decode::StageDesc*>(smem + kOffDesc), smem + kOffZero,
                                         mg_full, mg_empty,
-                                        reinterpret_cast<float*>(smem + kCtrlBytes + kOwnStages * p.own.stage_bytes),
-                                        plan.u1 - plan.u0, warp, lane);
+                                        reinterpret_cast<float*>(smem + kCtrlBytes + p.stages * p.own.stage_bytes),
+                                        plan.u1 - plan.u0, warp, lane, p.stages);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(bars.done());
@@ -1109,9 +1108,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (work) {
         if (!plan.shared)
-          decode::produce<kOwnStages, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
+          decode::produce<0, true>(own_q, own_k, own_v, own_k1, own_v1, p.own, smem + kCtrlBytes, full, empty,
                                             reinterpret_cast<decode::StageDesc*>(smem + kOffDesc), win, plan.u0,
-                                            plan.u1 - plan.u0, plan.at, plan.before, plan.c, maker ? 1 : 0, 2, lane);
+                                            plan.u1 - plan.u0, plan.at, plan.before, plan.c, maker ? 1 : 0, 2, lane,
+                                            p.stages);
         else if (warp == kWarpLoad)
           load_warp(tm_q, tm_k, tm_v, p, tab, smem, bars, w, e, pages, lane);
         else
@@ -1384,7 +1384,9 @@ extern "C" int la_paged_decode_shared_prefix(
     if ((st = encode_tensor_map_bf16(&tk, k_cache, 4, dims, strides, box, true)) != LA_OK) return st;
     if ((st = encode_tensor_map_bf16(&tv, v_cache, 4, dims, strides, box, true)) != LA_OK) return st;
   }
-  const size_t own = kCtrlBytes + static_cast<size_t>(kOwnStages) * call.p.stage_bytes + call.merge_bytes + 1024;
+  const size_t two = kCtrlBytes + 2 * static_cast<size_t>(call.p.stage_bytes) + call.merge_bytes + 1024;
+  p.stages = two + call.p.stage_bytes <= 227 * 1024 ? 3 : 2;
+  const size_t own = two + (p.stages - 2) * static_cast<size_t>(call.p.stage_bytes);
   const size_t smem = own > kSmemBytes ? own : kSmemBytes;
   if (smem > 227 * 1024) return LA_ERR_UNSUPPORTED;
   st = cuda_status(launch_pdl(shared_prefix_kernel, dim3(grid), dim3(kThreads), smem, stream, tq, tk, tv, call.q, call.k,
