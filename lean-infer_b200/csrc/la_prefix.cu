@@ -10,14 +10,21 @@
 //
 // shared_prefix_kernel does both at once, each on its own SMs. The shared part
 // is bound by the tensor cores and the exponentials when many rows share a
-// prefix (a step, see below, takes ~2.4 us on an SM); the rows' own keys are
-// bound by HBM, which about 64 SMs of streaming CTAs already draw 4.75 of its
-// ~6 TB/s from (96: 5.7). One after the other on all SMs, the two took their
-// sum, and each its own start (128 rows behind 32768 keys: 103 us); side by
-// side they take little more than the longer one. Every CTA counts the steps
-// and units of both parts and takes the same decision: P CTAs for the prefixes,
-// as many as finish with the rest by this model, the others for the rows.
-// combine_kernel joins the parts of every row.
+// prefix: a step (see below) is 2048 cycles of products and as many of
+// exponentials on an SM and takes ~2.2 us (128 rows with 32768 shared keys only:
+// 51 us, 0.67 PFLOP/s of products). The rows' own keys are bound by HBM, which
+// about 64 SMs of streaming CTAs already draw 4.75 of its ~6 TB/s from (96: 5.7).
+// One after the other on all SMs, the two took their sum, and each its own start
+// (128 rows behind 32768 keys: 103 us); side by side they take little more than
+// the longer one (62 us, 71 once the power limit has lowered the clock). Every CTA
+// counts the steps and units of both parts and takes the same decision: P CTAs
+// for the prefixes, as many as finish with the rest by a model of both, the
+// others for the rows. combine_kernel joins the parts of every row.
+//
+// 128 rows, 16 query and 8 kv heads, mostly their own keys behind 2048 shared
+// ones: 50.3 us, 88 % of HBM's measured rate; 4 rows: 11 us, of which ~4 pass
+// before the plan is there and checked and ~3 between the last CTA's end and the
+// combined row (instructions that run once cost ~10 ns each, from a cold cache).
 //
 // Shared part. For one kv head the group's rows x query heads of the kv head
 // are the rows of Q; with 128-key tiles of K and V,
@@ -28,15 +35,18 @@
 // accumulators take the even and the odd key tiles instead, so that one
 // tile's products still run while the other's exponentials do. A step is two
 // tile products either way: one key tile of a pair of row tiles, or two key
-// tiles of a single one. The steps of all items, laid end to end, are cut into
-// P equal ranges; an item's part in a range is a segment, which leaves
-// normalised fp32 O rows and base-2 logarithms of its sums.
+// tiles of a single one. S and P go in halves of 64 keys, so that a tile's
+// softmax of one half runs while the products of the other do (whole tiles:
+// 80.6 us instead of 72.5 for 128 rows behind 32768 keys, although a product of
+// half the width takes three quarters of the time). The steps of all items, laid
+// end to end, are cut into P equal ranges; an item's part in a range is a
+// segment, which leaves normalised fp32 O rows and base-2 logarithms of its sums.
 //
 // CTA, 12 warps. Shared part: 0-3 and 4-7 softmax of tile 0 and 1 (a thread
-// per row, the S row in registers), which store the segments' O as well, 8
-// issues the products, 9 the TMA loads; tensor memory holds S0 S1 O0 O1, 128
-// columns each, P over S. Own keys: 0-7 consume, 10 and 11 load. 10 makes the
-// plan.
+// per row, half a tile's S row in registers), which store the segments' O as
+// well, 8 and 11 issue the products of tile 0 and 1, 9 the TMA loads; tensor
+// memory holds S0 S1 O0 O1, 128 columns each, P over S. Own keys: 0-7 consume,
+// 10 and 11 load. 10 makes the plan.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
