@@ -306,7 +306,7 @@ def flash_attn_with_shared_prefix(
            and cache_seqlens.device == device and prefix_lens.device == device and cu_prefix_rows.device == device,
            "all tensors must be on one device")
     dev = _device_index(q)
-    out = torch.empty((B, 1, Hq, D), dtype=torch.bfloat16, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=device) if return_softmax_lse else None
     if B > 0:
         size = _shared_prefix_workspace_bytes(dev, B, G, Hq, Hkv, D)
