@@ -63,8 +63,8 @@ namespace prefix {
 constexpr int kD = 128;
 constexpr int kRows = 128;             // query rows per tile
 constexpr int kKeys = 128;             // keys per K/V tile
-constexpr int kParts = 2;
-constexpr int kPart = kKeys / kParts;
+constexpr int kParts = 2;              // S and P of a key tile
+constexpr int kPart = kKeys / kParts;  // keys of each
 constexpr int kHalf = 128 * 128;       // 64 dims of 128 rows: 16 KB
 constexpr int kTile = 2 * kHalf;
 constexpr int kStages = 4;             // K/V tiles in flight
@@ -660,10 +660,8 @@ __device__ __forceinline__ void softmax_warp(const Params& p, const PrefixGroup*
       // next waits for this P. (The one but last is done, since S was issued
       // behind it: the parity means the last.)
       if (j >= 1 && __any_sync(0xffffffffu, m_new != m)) {
-        if (kParts > 1) {
-          if (!(ok = wait_all(pv_done, (seen - 1) & 1))) break;
-          tc_fence_after();
-        }
+        if (!(ok = wait_all(pv_done, (seen - 1) & 1))) break;
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float o[32];

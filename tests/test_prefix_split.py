@@ -126,3 +126,18 @@ def test_segments_and_partial_rows(seed):
         got = s.reads(b, hh)
         assert len(got) == len(set(got)) and set(got) == rows
     assert {b for b, _ in want} == {b for f, n, k in groups if n >= 2 and k for b in range(f, f + n)}
+
+
+@pytest.mark.parametrize("grid", [2, 3, 7, 8, 64, 131, 132, 147, 148])
+def test_every_part_of_the_division_is_taken_once(grid):
+    """take_part: with Q CTAs (an even number) that stream, the others' numbers
+    are 0..grid-Q-1, theirs 0..Q-1, and neighbours 2i, 2i+1 have the same part."""
+    pairs = grid // 2
+    for Q in range(0, grid + 1 - (grid & 1) if grid > 2 else 2, 2):
+        half, got = Q // 2, {True: [], False: []}
+        for block in range(grid):
+            pair = block // 2
+            before = pair * half // pairs
+            shared = pair >= pairs or (pair + 1) * half // pairs == before
+            got[shared].append(block - 2 * min(before, half) if shared else 2 * before + (block & 1))
+        assert sorted(got[False]) == list(range(Q)) and sorted(got[True]) == list(range(grid - Q)), (grid, Q)
