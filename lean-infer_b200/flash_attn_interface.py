@@ -278,46 +278,52 @@ def flash_attn_with_shared_prefix(
     Its workspace is allocated per call, so calls may overlap.
     """
     # A decode step calls this once per layer, and a small batch is through on
-    # the GPU in some 11 us: each attribute is fetched once, addresses are
-    # passed as plain integers.
+    # the GPU in some 11 us: each attribute is fetched once, the checks are plain
+    # ifs, addresses are passed as plain integers.
     q_shape, kv_shape, q_stride, kv_stride = q.shape, k_cache.shape, q.stride(), k_cache.stride()
-    _check(len(q_shape) == 4 and q_shape[1] == 1, "q must be [batch, 1, num_heads, head_dim]")
-    _check(len(kv_shape) == 4 and kv_shape == v_cache.shape and kv_stride == v_cache.stride(),
-           "k_cache and v_cache must be [num_blocks, block_size, num_heads_k, head_dim] of the same strides")
+    if len(q_shape) != 4 or q_shape[1] != 1:
+        raise RuntimeError("q must be [batch, 1, num_heads, head_dim]")
+    if len(kv_shape) != 4 or kv_shape != v_cache.shape or kv_stride != v_cache.stride():
+        raise RuntimeError("k_cache and v_cache must be [num_blocks, block_size, num_heads_k, head_dim] of the same "
+                           "strides")
     B, _, Hq, D = q_shape
     NB, BS, Hkv, D_kv = kv_shape
-    _check(q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16,
-           "q, k_cache and v_cache must be bfloat16")
-    _check(q_stride[3] == 1 and kv_stride[3] == 1, "the head_dim axis must be contiguous")
-    _check(D_kv == D, "head_dim of q and k_cache differ")
-    _check(Hkv > 0 and Hq % Hkv == 0, "num_heads must be a multiple of num_heads_k")
-    bt_shape, (bt_row, bt_col) = block_table.shape, block_table.stride() if block_table.dim() == 2 else (0, 0)
-    _check(block_table.dtype is torch.int32 and len(bt_shape) == 2 and bt_shape[0] == B and bt_col == 1,
-           "block_table must be row-contiguous int32 [batch, max_blocks]")
-    _check(cache_seqlens.dtype is torch.int32 and cache_seqlens.shape == (B,) and cache_seqlens.is_contiguous(),
-           "cache_seqlens must be a contiguous int32 [batch] tensor")
-    _check(cu_prefix_rows.dtype is torch.int32 and cu_prefix_rows.dim() == 1 and cu_prefix_rows.numel() >= 1
-           and cu_prefix_rows.is_contiguous(), "cu_prefix_rows must be a contiguous int32 [groups + 1] tensor")
-    G = cu_prefix_rows.numel() - 1
-    _check(prefix_lens.dtype is torch.int32 and prefix_lens.shape == (G,) and prefix_lens.is_contiguous(),
-           "prefix_lens must be a contiguous int32 [groups] tensor")
-    device = q.device
-    _check(k_cache.device == device and v_cache.device == device and block_table.device == device
-           and cache_seqlens.device == device and prefix_lens.device == device and cu_prefix_rows.device == device,
-           "all tensors must be on one device")
+    bf16, i32 = torch.bfloat16, torch.int32
+    if q.dtype is not bf16 or k_cache.dtype is not bf16 or v_cache.dtype is not bf16:
+        raise RuntimeError("q, k_cache and v_cache must be bfloat16")
+    if q_stride[3] != 1 or kv_stride[3] != 1:
+        raise RuntimeError("the head_dim axis must be contiguous")
+    if D_kv != D:
+        raise RuntimeError("head_dim of q and k_cache differ")
+    if Hkv <= 0 or Hq % Hkv != 0:
+        raise RuntimeError("num_heads must be a multiple of num_heads_k")
+    bt_shape, bt_stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not i32 or len(bt_shape) != 2 or bt_shape[0] != B or bt_stride[1] != 1:
+        raise RuntimeError("block_table must be row-contiguous int32 [batch, max_blocks]")
+    if cache_seqlens.dtype is not i32 or cache_seqlens.shape != (B,) or not cache_seqlens.is_contiguous():
+        raise RuntimeError("cache_seqlens must be a contiguous int32 [batch] tensor")
+    cu_shape = cu_prefix_rows.shape
+    if cu_prefix_rows.dtype is not i32 or len(cu_shape) != 1 or cu_shape[0] < 1 or not cu_prefix_rows.is_contiguous():
+        raise RuntimeError("cu_prefix_rows must be a contiguous int32 [groups + 1] tensor")
+    G = cu_shape[0] - 1
+    if prefix_lens.dtype is not i32 or prefix_lens.shape != (G,) or not prefix_lens.is_contiguous():
+        raise RuntimeError("prefix_lens must be a contiguous int32 [groups] tensor")
     dev = _device_index(q)
+    if not (k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cache_seqlens.get_device()
+            == prefix_lens.get_device() == cu_prefix_rows.get_device() == dev):
+        raise RuntimeError("all tensors must be on one device")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=device) if return_softmax_lse else None
+    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=q.device) if return_softmax_lse else None
     if B > 0:
         size = _shared_prefix_workspace_bytes(dev, B, G, Hq, Hkv, D)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         with torch.cuda.device(dev):
             ensure_init(dev)
             _lib.call(
                 "la_paged_decode_shared_prefix",
                 q.data_ptr(), q_stride[0], q_stride[2],
                 k_cache.data_ptr(), v_cache.data_ptr(), kv_stride[0], kv_stride[1], kv_stride[2], NB, BS,
-                block_table.data_ptr(), bt_row, bt_shape[1],
+                block_table.data_ptr(), bt_stride[0], bt_shape[1],
                 cache_seqlens.data_ptr(),
                 prefix_lens.data_ptr(), cu_prefix_rows.data_ptr(), G,
                 B, Hq, Hkv, D,
