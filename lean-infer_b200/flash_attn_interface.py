@@ -308,15 +308,15 @@ def flash_attn_with_shared_prefix(
     G = cu_shape[0] - 1
     if prefix_lens.dtype is not i32 or prefix_lens.shape != (G,) or not prefix_lens.is_contiguous():
         raise RuntimeError("prefix_lens must be a contiguous int32 [groups] tensor")
-    dev = _device_index(q)
+    dev = q.get_device() if q.is_cuda else _device_index(q)
     if not (k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cache_seqlens.get_device()
             == prefix_lens.get_device() == cu_prefix_rows.get_device() == dev):
         raise RuntimeError("all tensors must be on one device")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=q.device) if return_softmax_lse else None
+    lse = q.new_empty((B, Hq, 1), dtype=torch.float32) if return_softmax_lse else None
     if B > 0:
         size = _shared_prefix_workspace_bytes(dev, B, G, Hq, Hkv, D)
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        workspace = cache_seqlens.new_empty((size + 3) // 4)
         with torch.cuda.device(dev):
             ensure_init(dev)
             _lib.call(
