@@ -557,6 +557,7 @@ struct Bars {
   __device__ __forceinline__ uint64_t* planned() const { return b + 24; }  // the plan is in shared memory
   __device__ __forceinline__ uint64_t* checked() const { return b + 25; }  // it was checked after the wait
   __device__ __forceinline__ uint64_t* done() const { return b + 26; }     // a softmax warp is through (8)
+  __device__ __forceinline__ uint64_t* again() const { return b + 27; }    // a warp has left the stale plan (11)
 };
 
 __device__ __forceinline__ bool wait_warp(const Params& p, uint64_t* bar, uint32_t parity) {
@@ -995,6 +996,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bars.planned(), 1);
     mbar_init(bars.checked(), 1);
     mbar_init(bars.done(), 8);
+    mbar_init(bars.again(), kThreads / 32 - 1);
     for (int s = 0; s < 3; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], decode::kCWarps);
@@ -1027,11 +1029,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (!early) grid_dependency_wait();
 
   // Round 0 with the plan; before anything is done by it, the check has to be
-  // back. If the plan was stale, round 1 with the new one.
+  // back. If the plan was stale, round 1 with the new one, which is made when
+  // all warps have left the old one.
   // (A round through each warp's code before the plan was there, to fetch it
   // into the instruction caches, made every size 3 to 35 % slower.)
+  auto leave_plan = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars.again());
+  };
   if (warp < 8) {
     bool ok = false;
     for (uint32_t round = 0; round < 2; ++round) {
@@ -1040,7 +1048,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (round == 0) {
         if (!wait_warp(p, bars.checked(), 0)) break;
         if (*stale) {
-          named_sync(1, kThreads);
+          leave_plan();
           continue;
         }
       }
@@ -1067,7 +1075,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     win.tab = tab;
     for (uint32_t round = 0; round < 2; ++round) {
       if (maker) {
-        if (round == 0 && !early) grid_dependency_wait();
         const Plan r = early ? make_plan(p, tab, in, lane) : make_large_plan(p, tab, lane);
         if (lane == 0) {
           plan = r;
@@ -1110,7 +1117,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (round == 0) {
         if (!wait_warp(p, bars.checked(), 0)) break;
         if (*stale) {
-          named_sync(1, kThreads);
+          if (!maker)
+            leave_plan();
+          else if (!wait_warp(p, bars.again(), 0))
+            break;
           continue;
         }
       }
