@@ -16,7 +16,7 @@
 // about 64 SMs of streaming CTAs already draw 4.75 of its ~6 TB/s from (96: 5.7).
 // One after the other on all SMs, the two took their sum, and each its own start
 // (128 rows behind 32768 keys: 103 us); side by side they take little more than
-// the longer one (62 us, 71 once the power limit has lowered the clock). Every CTA
+// the longer one (62 us, 72 once the power limit has lowered the clock). Every CTA
 // counts the steps and units of both parts and takes the same decision: P CTAs
 // for the prefixes, as many as finish with the rest by a model of both, the
 // others for the rows. combine_kernel joins the parts of every row.
