@@ -1344,8 +1344,9 @@ extern "C" int la_paged_decode_shared_prefix(
   if (st != LA_OK || batch == 0) return st;
   if (num_blocks > 0x7ffffffeLL) return LA_ERR_UNSUPPORTED;
   const int device = current_device();
-  const int grid = device >= 0 ? num_sms(device) : 0;
+  const int grid = device >= 0 ? num_sms(device) & ~1 : 0;  // take_part and shared_ctas deal in pairs
   if (grid <= 0) return LA_ERR_CUDA;
+  if (grid < 4) return LA_ERR_UNSUPPORTED;  // a pair for each part
   const Workspace w = workspace_of(batch, num_q_heads, num_kv_heads, grid);
   if (w.rows > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return LA_ERR_WORKSPACE;
