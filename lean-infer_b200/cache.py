@@ -106,19 +106,20 @@ def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple:
     """The pools as la_copy_blocks takes them, from [L, NB, BS, Hkv, D] or one
     layer's [NB, BS, Hkv, D]."""
     shape, stride = k_pool.shape, k_pool.stride()
-    _check(len(shape) in (4, 5) and shape == v_pool.shape and stride == v_pool.stride()
-           and k_pool.dtype is v_pool.dtype and k_pool.device == v_pool.device,
-           "k_pool and v_pool must be [num_layers, num_blocks, block_size, num_heads_k, head_dim] (or one layer) of the "
-           "same shape, strides and type on one device")
-    _check(stride[-1] == 1, "the head_dim axis must be contiguous")
-    layers, layer_stride = (shape[0], stride[0]) if len(shape) == 5 else (1, 0)
-    return (k_pool.data_ptr(), v_pool.data_ptr(), layer_stride, *stride[-4:-1], layers, *shape[-4:],
-            k_pool.element_size())
+    if (len(shape) not in (4, 5) or shape != v_pool.shape or stride != v_pool.stride()
+            or k_pool.dtype is not v_pool.dtype or k_pool.get_device() != v_pool.get_device()):
+        raise RuntimeError("k_pool and v_pool must be [num_layers, num_blocks, block_size, num_heads_k, head_dim] (or one "
+                           "layer) of the same shape, strides and type on one device")
+    if stride[-1] != 1:
+        raise RuntimeError("the head_dim axis must be contiguous")
+    if len(shape) == 4:
+        return (k_pool.data_ptr(), v_pool.data_ptr(), 0, *stride[:3], 1, *shape, k_pool.element_size())
+    return (k_pool.data_ptr(), v_pool.data_ptr(), *stride[:4], *shape, k_pool.element_size())
 
 
-def _ids(name: str, ids: torch.Tensor, n: int, device: torch.device) -> int:
-    _check(ids.dtype is torch.int32 and ids.shape == (n,) and ids.is_contiguous() and ids.device == device,
-           f"{name} must be a contiguous int32 [num_pairs] tensor on the pools' device")
+def _ids(name: str, ids: torch.Tensor, n: int, dev: int) -> int:
+    if ids.dtype is not torch.int32 or ids.shape != (n,) or not ids.is_contiguous() or ids.get_device() != dev:
+        raise RuntimeError(f"{name} must be a contiguous int32 [num_pairs] tensor on the pools' device")
     return ids.data_ptr()
 
 
@@ -141,10 +142,10 @@ def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Te
     of one before it, is skipped and recorded, as are ids outside the pool
     (check_device_errors)."""
     args = _pools(k_pool, v_pool)
-    device, n = k_pool.device, src_blocks.numel()
-    dev = _device_index(k_pool)
-    src, dst = _ids("src_blocks", src_blocks, n, device), _ids("dst_blocks", dst_blocks, n, device)
-    tokens = _ids("num_tokens", num_tokens, n, device) if num_tokens is not None else None
+    n = src_blocks.numel()
+    dev = k_pool.get_device() if k_pool.is_cuda else _device_index(k_pool)
+    src, dst = _ids("src_blocks", src_blocks, n, dev), _ids("dst_blocks", dst_blocks, n, dev)
+    tokens = _ids("num_tokens", num_tokens, n, dev) if num_tokens is not None else None
     with torch.cuda.device(dev):
         ensure_init(dev)
         _lib.call("la_copy_blocks", *args, src, dst, tokens, n, error_word(dev).data_ptr(), _raw_stream(dev))
@@ -157,10 +158,10 @@ def move_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Te
     rewritten in place) becomes dst_blocks[i]. Entries of a move that is
     skipped (see copy_blocks) stay as they are."""
     args = _pools(k_pool, v_pool)
-    device, n = k_pool.device, src_blocks.numel()
-    dev = _device_index(k_pool)
-    src, dst = _ids("src_blocks", src_blocks, n, device), _ids("dst_blocks", dst_blocks, n, device)
-    _check_table(block_table, device)
+    n = src_blocks.numel()
+    dev = k_pool.get_device() if k_pool.is_cuda else _device_index(k_pool)
+    src, dst = _ids("src_blocks", src_blocks, n, dev), _ids("dst_blocks", dst_blocks, n, dev)
+    _check_table(block_table, k_pool.device)
     rows, cols = block_table.shape
     with torch.cuda.device(dev):
         ensure_init(dev)
