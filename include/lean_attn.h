@@ -277,7 +277,8 @@ int la_paged_decode_noalloc(
  * The same result as la_paged_decode on the same arguments, with the keys of
  * a shared prefix read once for all the rows that share it. Rows
  * cu_prefix_rows[g] .. cu_prefix_rows[g+1]-1 (int32 [num_groups + 1], not
- * decreasing, within 0..batch, else LA_DEVERR_PREFIX) form group g: their
+ * decreasing, within 0..batch; else LA_DEVERR_PREFIX is set and no rows share:
+ * each reads all its keys by itself, to the same result) form group g: their
  * block tables name the same pages for keys 0..prefix_lens[g]-1 (int32
  * [num_groups]), and those are read through the table of the group's first
  * row. Only whole pages are taken as shared: prefix_lens[g] is rounded down to

@@ -24,12 +24,19 @@ struct PrefixGroup {
   int first, rows, keys;
 };
 
+// Bounds that run backwards can make groups overlap that are runs of rows each
+// for itself, and no two warps need agree on whose a row is then. So where one
+// group is no run of the batch's rows, all are empty, and every row reads its
+// keys by itself.
+__device__ __forceinline__ bool run_of_rows(const PrefixGroups& G, int first, int last) {
+  return first >= 0 && first <= last && last <= G.batch;
+}
+
 __device__ __forceinline__ PrefixGroup group_from(const PrefixGroups& G, int first, int last, int len) {
   PrefixGroup r;
   r.first = first;
   const long long n = min(static_cast<long long>(max(len, 0)), G.cap);
-  const bool sound = r.first >= 0 && r.first <= last && last <= G.batch;
-  r.rows = sound ? last - r.first : 0;
+  r.rows = run_of_rows(G, first, last) ? last - r.first : 0;
   const int blocks = G.bs_shift >= 0 ? static_cast<int>(n) >> G.bs_shift : static_cast<int>(n) / G.block_size;
   r.keys = r.rows >= 2 ? blocks * G.block_size : 0;
   return r;
@@ -40,9 +47,14 @@ __device__ __forceinline__ PrefixGroup load_group(const PrefixGroups& G, int g) 
   return group_from(G, __ldcg(G.cu + g), __ldcg(G.cu + g + 1), __ldcg(G.lens + g));
 }
 
-// From the CTA's table of all groups, where there is room for one.
+// The CTA's table: up to kMaxGroups groups. Of more, which are read where they
+// are needed, its first entry says whether all are runs of rows (rows: 1 or 0).
+constexpr int kMaxGroups = 512;
 __device__ __forceinline__ PrefixGroup prefix_group(const PrefixGroups& G, const PrefixGroup* tab, int g) {
-  return tab ? tab[g] : load_group(G, g);
+  if (G.n <= kMaxGroups) return tab[g];
+  PrefixGroup r = load_group(G, g);
+  if (tab->rows == 0) r.rows = r.keys = 0;
+  return r;
 }
 
 // Keys of row b that its group's pass covers; the row reads those behind them
@@ -53,7 +65,7 @@ __device__ __forceinline__ int prefix_keys(const PrefixGroups& G, const PrefixGr
   int lo = -1, hi = G.n;  // the last group that begins at or before row b
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((tab ? tab[mid].first : G.cu[mid]) <= b)
+    if ((G.n <= kMaxGroups ? tab[mid].first : G.cu[mid]) <= b)
       lo = mid;
     else
       hi = mid;

@@ -85,7 +85,6 @@ constexpr int kOffZero = 640;
 constexpr int kOffWalk = 768;          // of the softmax warps, kept out of their registers
 constexpr int kWalkBytes = 120;
 constexpr int kOffTable = 2048;
-constexpr int kMaxGroups = 512;        // groups that the table holds; more are read from global memory
 constexpr int kCtrlBytes = 8192;
 constexpr int kOffQ = kCtrlBytes;
 constexpr int kOffKV = kOffQ + 2 * kTile;
@@ -323,8 +322,9 @@ __device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, con
   const PrefixGroups& G = p.own.groups;
   PrefixGroup grp{0, 0, 0};
   Shape h{0, 0, 0, 0, 0};
+  const bool sound = __all_sync(0xffffffffu, lane >= G.n || run_of_rows(G, in.lo, in.hi));
   if (lane < G.n) {
-    grp = group_from(G, in.lo, in.hi, in.len);
+    if (sound) grp = group_from(G, in.lo, in.hi, in.len);
     tab[lane] = grp;
     if (grp.keys > 0) h = shape_of(p, grp);
   }
@@ -369,26 +369,35 @@ __device__ __forceinline__ Plan make_plan(const Params& p, PrefixGroup* tab, con
   return r;
 }
 
-// The same for any number of rows and groups. tab: the table to fill, or null
-// where the groups exceed it.
+// The same for any number of rows and groups.
 __device__ __noinline__ Plan make_large_plan(const Params& p, PrefixGroup* tab, int lane) {
   const PrefixGroups& G = p.own.groups;
   int raw[8];
   long long S = 0, single = 0, U = 0;
   int items = 0;
   const PrefixGroup none{0, 0, 0};
+  bool sound = true;
   for (int b = 0; b < G.n; b += 32) {
     const int g = b + lane;
     Shape h{0, 0, 0, 0, 0};
     if (g < G.n) {
-      const PrefixGroup r = load_group(G, g);
-      if (tab) tab[g] = r;
+      const int lo = __ldcg(G.cu + g), hi = __ldcg(G.cu + g + 1);
+      const PrefixGroup r = group_from(G, lo, hi, __ldcg(G.lens + g));
+      sound &= run_of_rows(G, lo, hi);
+      if (G.n <= kMaxGroups) tab[g] = r;
       if (r.keys > 0) h = shape_of(p, r);
     }
     S += warp_sum(p.own.hkv * h.per_head);
     single += warp_sum(p.own.hkv * h.half);
     items += warp_sum(h.tiles ? p.own.hkv * h.pairs : 0);
   }
+  sound = __all_sync(0xffffffffu, sound);
+  if (!sound) {
+    S = single = 0;
+    items = 0;
+    for (int g = lane; g < min(G.n, kMaxGroups); g += 32) tab[g] = none;
+  }
+  if (G.n > kMaxGroups && lane == 0) tab->rows = sound;
   __syncwarp();
   for (int base = 0; base < G.batch; base += 256) {
     load_lens8(p, lane, base, raw);
@@ -971,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + decode::kMaxStages;
   uint64_t* mg_full = empty + decode::kMaxStages;  // all consumer warps wrote their state
   uint64_t* mg_empty = mg_full + 1;                // the merging warp read it
-  PrefixGroup* tab = p.own.groups.n <= kMaxGroups ? reinterpret_cast<PrefixGroup*>(smem + kOffTable) : nullptr;
+  PrefixGroup* tab = reinterpret_cast<PrefixGroup*>(smem + kOffTable);
   Plan& plan = *reinterpret_cast<Plan*>(smem + kOffPlan);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;

@@ -273,7 +273,9 @@ def flash_attn_with_shared_prefix(
     list of tables. Only whole blocks are taken as shared (prefix_lens is
     rounded down). Rows in no group, empty groups and rows that end inside
     the prefix are fine. All of it is read on the device: a captured graph
-    serves any division of the batch into at most G groups.
+    serves any division of the batch into at most G groups. Where
+    cu_prefix_rows descends or leaves the batch, that is recorded
+    (check_device_errors) and every row reads all its keys by itself.
     Returns out [B, 1, Hq, D] (and softmax_lse [B, Hq, 1] fp32 when asked).
     Its workspace is allocated per call, so calls may overlap.
     """

@@ -391,3 +391,18 @@ def test_refusals(pkg, cuda_dev):
         f(w.q[..., :64], w.k[..., :64], w.v[..., :64], w.lens, w.table, w.prefix, w.cu)
     with pytest.raises(RuntimeError, match="invalid argument"):
         f(w.q, w.k, w.v, w.lens, w.table, w.prefix, w.cu, softmax_scale=-1.0)
+
+
+@pytest.mark.parametrize("cu", [[0, 100, 50, 128], [10, 60, 20, 70, 30, 128], [0, 128, 0, 128], [0, 2, 99, 300], [-1, 64, 128]])
+@pytest.mark.parametrize("more_groups,more_rows", [(0, 0), (40, 0), (600, 0), (0, 150)])
+def test_rows_are_right_whatever_the_bounds(pkg, cuda_dev, cu, more_groups, more_rows):
+    """Bounds that run backwards or leave the batch, some with runs of rows that
+    overlap, are reported, no rows share, and every row has its own result."""
+    w = Batch(cuda_dev, [(128, 512)], own(128 + more_rows, -200, 100), 128, 4, 2, seed=20)
+    cu = cu + [cu[-1]] * more_groups
+    w.cu = torch.tensor(cu, dtype=torch.int32, device=cuda_dev)
+    w.prefix = torch.full((len(cu) - 1,), 512, dtype=torch.int32, device=cuda_dev)
+    got = w.call(pkg)
+    with pytest.raises(RuntimeError, match="prefix groups"):
+        pkg.check_device_errors(cuda_dev.index)
+    w.check(pkg, got)
