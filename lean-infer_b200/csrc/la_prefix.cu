@@ -1085,6 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t round = 0; round < 2; ++round) {
       if (maker) {
         const Plan r = early ? make_plan(p, tab, in, lane) : make_large_plan(p, tab, lane);
+        __syncwarp();  // the entries of `tab` are all lanes' stores, lane 0 arrives for them
         if (lane == 0) {
           plan = r;
           mbar_arrive(bars.planned());

@@ -105,3 +105,14 @@ def test_random_bounds(divide, seed):
         cu[r.randrange(n + 1)] = r.randint(-2, batch + 2)
     lens = [r.choice((0, bs, r.randint(-3, 3000), 10 ** 9)) for _ in range(n)]
     _check(divide, cu, lens, batch, bs, 2048 // bs * bs, [r.randint(0, 2048) for _ in range(batch)])
+
+
+def test_all_lanes_entries_are_published_with_the_plan():
+    """Every lane fills entries of the table, one lane arrives for all of them.
+    Shuffles and votes between do not order memory: the other lanes' stores are
+    published only if the warp synchronises before that lane arrives."""
+    text = (REPO / "lean-infer_b200" / "csrc" / "la_prefix.cu").read_text()
+    made = text.index("make_plan(p, tab, in, lane)")
+    published = text.index("mbar_arrive(bars.planned())", made)
+    assert text[made:published].count("__syncwarp();") == 1
+    assert text.index("__syncwarp();", made) < text.index("if (lane == 0)", made) < published
