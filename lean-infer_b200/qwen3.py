@@ -402,9 +402,11 @@ class BucketedDecodeGraph:
 
     def capture(self) -> None:
         """Three warm-up forwards per bucket on a side stream, then one graph
-        per bucket (all rows idle while capturing: nothing is written)."""
+        per bucket (all rows idle while capturing: nothing is written, and no
+        rows share, since a step's groups may exceed a smaller bucket)."""
         self.pos.fill_(-1)
         self.ctx.zero_()
+        self._dev_prefix.zero_()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
