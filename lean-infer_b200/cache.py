@@ -75,12 +75,19 @@ class BlockAllocator:
         return self._holders.get(block, 0)
 
     def release(self, blocks: list[int]) -> None:
+        """One holder less for each of `blocks`; those that nobody holds any
+        more go to the tail of the free list. Refused as a whole where a block
+        has fewer holders than that: it would be handed out twice."""
+        left: dict[int, int] = {}
         for b in blocks:
-            n = self._holders.get(b, 1) - 1
-            if n > 0:
-                self._holders[b] = n
-            else:
-                self._holders.pop(b, None)
+            left[b] = left.get(b, self._holders.get(b, 0)) - 1
+        over = [b for b, n in left.items() if n < 0]
+        if over:
+            raise ValueError(f"blocks {over} are released more often than they are held")
+        for b in blocks:
+            self._holders[b] -= 1
+            if self._holders[b] == 0:
+                del self._holders[b]
                 self.free.append(b)
 
     def compact(self) -> tuple[list[int], list[int]]:

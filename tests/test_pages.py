@@ -207,3 +207,20 @@ def test_staged_prefix_groups(pkg):
     for bad in (([1] * 5, list(range(6))), ([1], [0, 9]), ([1, 1], [0, 4, 2]), ([1], [0]), ([1], [-1, 2])):
         with pytest.raises(ValueError):
             qwen3.stage_prefix(lens, cu, bad, 8)
+
+
+@pytest.mark.parametrize("again", [[1], [2], [0], [9], [3, 3], [3, 1], [4, 4, 4]])
+def test_allocator_refuses_a_release_too_many(pkg, again):
+    """A block released more often than it is held would be handed out to two
+    sequences; block 0 is nobody's. Nothing of a refused call is done."""
+    a = pkg.BlockAllocator(6)
+    x = a.allocate(4)  # 1, 2, 3, 4
+    a.fork([4])
+    a.release([1, 2])
+    with pytest.raises(ValueError, match="released"):
+        a.release(again)
+    assert [a.holders(b) for b in x] == [0, 0, 1, 2] and list(a.free) == [5, 1, 2]
+    a.release([4, 3, 4])  # its two holders in one call
+    assert list(a.free) == [5, 1, 2, 3, 4] and a.compact() == ([], [])
+    got = a.allocate(5)
+    assert sorted(got) == [1, 2, 3, 4, 5] and a.num_free == 0
