@@ -177,30 +177,65 @@ def move_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: torch.Te
                   error_word(dev).data_ptr(), _raw_stream(dev))
 
 
+def _common_blocks(a: list[int], b: list[int]) -> int:
+    """Blocks that two rows begin with."""
+    n = min(len(a), len(b))
+    if a[:n] == b[:n]:
+        return n
+    same, differ = 0, n  # a[:same] and b[:same] are the same, a[:differ] and b[:differ] differ
+    while differ - same > 1:
+        mid = (same + differ) // 2
+        if a[same:mid] == b[same:mid]:
+            same = mid
+        else:
+            differ = mid
+    return same
+
+
 def shared_prefix_groups(tables: Sequence[Sequence[int]], lengths: Sequence[int], block_size: int,
                          min_blocks: int = 1) -> tuple[list[int], list[int]]:
     """The groups that flash_attn_with_shared_prefix takes, from the rows'
-    block tables: (prefix_lens, cu_prefix_rows). Consecutive rows whose tables
-    begin with the same block, filled by both, are one group; its prefix is
-    the run of blocks that all of them begin with and fill. Every row is in a
-    group: one that shares fewer than min_blocks blocks with its neighbours is
-    a group by itself, with a prefix of 0."""
-    lens, cu = [], [0]
-    rows = [list(t[: n // block_size]) for t, n in zip(tables, lengths)]
-    first = 0
-    while first < len(rows):
-        common, last = len(rows[first]), first + 1
-        while last < len(rows):
-            n = 0
-            while n < min(common, len(rows[last])) and rows[last][n] == rows[first][n]:
-                n += 1
-            if n < max(min_blocks, 1):
+    block tables: (prefix_lens, cu_prefix_rows). A group is a run of rows whose
+    tables begin with the same blocks, filled by all of them; its prefix is as
+    many of those as all have. Where rows share more with some neighbours than
+    with others (one system prompt, several documents behind it), the rows are
+    divided so that the fewest blocks are read, a prefix once for its group and
+    the other blocks once for each row; every group counts as one block read
+    for what it costs by itself. Every row is in a group: one that shares fewer
+    than min_blocks blocks with its neighbours is a group by itself, with a
+    prefix of 0."""
+    least = max(min_blocks, 1)
+    rows = [list(t[: max(n, 0) // block_size]) for t, n in zip(tables, lengths)]
+    n = len(rows)
+    # Blocks common to rows i - 1 and i; 0 where no group may reach across.
+    common = [0] + [_common_blocks(a, b) for a, b in zip(rows, rows[1:])] + [0]
+    common = [c if c >= least else 0 for c in common]
+    # Places where the best division may have to cut. Two rows that have as much
+    # in common as either has with its other neighbour stay together: of a cut
+    # between them, the row beside it on the side whose group shares less goes
+    # over to the other group, which goes on sharing as much, and saves no less.
+    cuts = [0] + [i for i in range(1, n) if common[i] == 0 or common[i] < max(common[i - 1], common[i + 1])] + [n]
+    every = 1 << 62
+    inside = [min(common[a + 1:b], default=every) for a, b in zip(cuts, cuts[1:])]
+    # best[j]: blocks saved, less groups made, of the rows before cuts[j]; last[j]: where their last group begins, its prefix
+    best, last = [0], [(0, 0)]
+    for j in range(1, len(cuts)):
+        shared, choices = every, []
+        for i in range(j - 1, -1, -1):
+            shared = min(shared, inside[i], common[cuts[i + 1]] if i + 1 < j else every)
+            if shared == 0:
                 break
-            common, last = n, last + 1
-        lens.append(common * block_size if last - first > 1 else 0)
-        cu.append(last)
-        first = last
-    return lens, cu
+            more = cuts[j] - cuts[i] - 1
+            choices.append((best[i] + more * shared - 1, -i, shared if more else 0))
+        saved, at, prefix = max(choices)
+        best.append(saved)
+        last.append((-at, prefix))
+    lens, cu, j = [], [n], len(cuts) - 1
+    while cu[-1] > 0:
+        j, prefix = last[j]
+        lens.append(prefix * block_size)
+        cu.append(cuts[j])
+    return lens[::-1], cu[::-1]
 
 
 class BlockCache:

@@ -224,3 +224,76 @@ def test_allocator_refuses_a_release_too_many(pkg, again):
     assert list(a.free) == [5, 1, 2, 3, 4] and a.compact() == ([], [])
     got = a.allocate(5)
     assert sorted(got) == [1, 2, 3, 4, 5] and a.num_free == 0
+
+
+def _reads(tables, lengths, bs, groups):
+    """Whole blocks that the rows read, the shared ones once for a group."""
+    lens, cu = groups
+    full = [n // bs for n in lengths]
+    assert cu[0] == 0 and cu[-1] == len(tables) and all(a < b for a, b in zip(cu, cu[1:]))
+    total = 0
+    for n, a, b in zip(lens, cu, cu[1:]):
+        assert n % bs == 0 and (b - a > 1 or n == 0)
+        k = n // bs
+        assert all(t[:k] == tables[a][:k] and f >= k for t, f in zip(tables[a:b], full[a:b]))
+        total += sum(full[a:b]) - (b - a - 1) * k
+    return total
+
+
+def _rows(*runs):
+    """Tables of (rows, blocks) runs that share a first block and, within the
+    run, the rest; each row ends with a block of its own."""
+    tables, ids = [], iter(range(10, 10 ** 6))
+    for n, k in runs:
+        mine = [1] + [next(ids) for _ in range(k - 1)]
+        tables += [mine + [next(ids)] for _ in range(n)]
+    return tables
+
+
+@pytest.mark.parametrize("runs,min_blocks,want", [
+    # a system prompt of one block in front of two documents, each asked several times
+    ([(64, 128), (64, 128)], 1, ([128, 128], [0, 64, 128])),
+    ([(4, 101), (4, 101)], 1, ([101, 101], [0, 4, 8])),
+    # one row that shares only the system prompt, behind and in front of and between the others
+    ([(64, 128), (1, 1)], 1, ([128, 0], [0, 64, 65])),
+    ([(1, 1), (64, 128)], 1, ([0, 128], [0, 1, 65])),
+    ([(9, 128), (1, 1), (9, 128)], 1, ([128, 0, 128], [0, 9, 10, 19])),
+    # so little beside it that a group of its own is not worth it
+    ([(2, 2), (6, 1)], 1, ([1], [0, 8])),
+    ([(2, 2), (6, 1)], 2, ([2] + [0] * 6, [0, 2, 3, 4, 5, 6, 7, 8])),
+])
+def test_shared_prefix_groups_keep_what_is_shared(pkg, runs, min_blocks, want):
+    tables, bs = _rows(*runs), 16
+    lens, cu = pkg.shared_prefix_groups(tables, [bs * len(t) - 3 for t in tables], bs, min_blocks)
+    assert ([n // bs for n in lens], cu) == want
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_shared_prefix_groups_against_every_division(pkg, seed):
+    """No division of the rows reads fewer blocks, a group counted as one."""
+    r = random.Random(seed)
+    bs, n, least = 16, r.randint(1, 8), r.choice((1, 1, 2))
+    tables, fresh = [], iter(range(100, 10 ** 4))
+    for _ in range(n):
+        keep = r.randint(0, len(tables[-1])) if tables else 0
+        tables.append((tables[-1][:keep] if keep else []) + [next(fresh) for _ in range(r.randint(0, 4))])
+    lengths = [r.randint(0, bs * len(t)) for t in tables]
+    best = None
+    for cuts in range(1 << (n - 1)):
+        cu = [0] + [i + 1 for i in range(n - 1) if cuts >> i & 1] + [n]
+        lens = []
+        for a, b in zip(cu, cu[1:]):
+            k = 0
+            while all(lengths[i] // bs > k and tables[i][k] == tables[a][k] for i in range(a, b)):
+                k += 1
+            lens.append(k * bs if b - a > 1 else 0)
+        if all(b - a == 1 or n >= least * bs for n, a, b in zip(lens, cu, cu[1:])):
+            cost = _reads(tables, lengths, bs, (lens, cu)) + len(lens)
+            best = cost if best is None else min(best, cost)
+    got = pkg.shared_prefix_groups(tables, lengths, bs, least)
+    assert _reads(tables, lengths, bs, got) + len(got[0]) == best
+    assert all(k == 0 or k >= least * bs for k in got[0])
+
+
+def test_shared_prefix_groups_of_lengths_below_zero(pkg):
+    assert pkg.shared_prefix_groups([[1, 2], [1, 2]], [-1, -40], 16) == ([0, 0], [0, 1, 2])
