@@ -206,3 +206,40 @@ def test_cache_fork_and_compact(pkg, cuda_dev):
     for t in kids:
         a.release(t)
     assert a.num_free == nb - 1
+
+
+def _us(f, before=lambda: None):
+    """Median time of a call on the device, `before` not counted."""
+    times = []
+    for _ in range(7):
+        before()
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1000)
+    return sorted(times)[3]
+
+
+def _scattered(r, total, n, dev):
+    """n pages of the upper half of the ids and their places in the lower."""
+    ids = sorted(r.sample(range(total), 2 * n))
+    return _i32(ids[n:], dev), _i32(ids[:n], dev), [b for b in range(total) if b not in set(ids[:n])]
+
+
+@pytest.mark.parametrize("n,rows,cols", [(1201, 131, 77), (6000, 128, 512)])
+def test_a_table_that_names_the_pages_takes_little_beside_the_copy(pkg, cuda_dev, n, rows, cols):
+    """Pages of 16 tokens in 7 layers, under a table most of whose entries name
+    one that moves: no more than twice the time of the copies."""
+    k, v = (torch.zeros(7, 2 * n + n // 3, 16, 8, 128, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2))
+    src, dst, used = _scattered(random.Random(n), k.shape[1], n, cuda_dev)
+    names = _i32(random.Random(1).choices(used, k=rows * cols), cuda_dev).view(rows, cols)
+    table = names.clone()
+    copy = _us(lambda: pkg.copy_blocks(k, v, src, dst))
+    move = _us(lambda: pkg.move_blocks(k, v, src, dst, table), lambda: table.copy_(names))
+    pkg.check_device_errors(cuda_dev.index)
+    to = torch.arange(k.shape[1], dtype=torch.int32, device=cuda_dev)
+    to[src.long()] = dst
+    assert torch.equal(table, to[names.long()])
+    assert move <= 2 * copy, (move, copy)
