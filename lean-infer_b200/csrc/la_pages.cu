@@ -37,7 +37,8 @@ struct Params {
   int token_units;  // of one token
   int flat;         // a page is one run of bytes (kFlat)
   int chunks;       // of a whole page
-  int pieces;       // layers, K and V
+  int parts;        // chunks of a pair in all tensors of all layers
+  int per;          // of them, those that one CTA copies
   long long num_blocks;
   const int* src;
   const int* dst;
@@ -61,7 +62,9 @@ __device__ __forceinline__ bool in_pool(const Params& p, int s, int d) {
 // One chunk of one pair in one tensor of one layer per CTA, the pairs in turn,
 // so that what runs at a time is spread over all their pages; CTAs behind a
 // partly filled page's tokens leave at once. The loads are issued before it is
-// known whether the pair meets another, the stores wait for that. Measured
+// known whether the pair meets another, the stores wait for that. To see it the
+// CTA reads all pairs, which is little beside its chunk up to some 1000 of them
+// (8 KB); behind that it copies more chunks of its pair (per_cta). Measured
 // (times of a copy at the rate of a plain tensor copy in brackets): 96 pages of
 // 28 layers 832 us (873), 64 partly filled ones 304 us (309), 3 pages 28.8 us
 // (27.3), one partly filled 9.5 us (8.2). 32 KB per CTA took up to 3 % longer,
@@ -71,11 +74,10 @@ __device__ __forceinline__ bool in_pool(const Params& p, int s, int d) {
 template <bool kFlat>
 __device__ __forceinline__ void copy_part(const Params& p, long long x) {
   const int i = static_cast<int>(x % p.n);
-  x /= p.n;
-  const int chunk = static_cast<int>(x % p.chunks), piece = static_cast<int>(x / p.chunks);
+  const int part0 = static_cast<int>(x / p.n) * p.per;
   const int tid = threadIdx.x;
   const int s = p.src[i], d = p.dst[i], n = p.tokens ? p.tokens[i] : p.block_size;
-  const bool first = piece == 0 && chunk == 0 && tid == 0;
+  const bool first = part0 == 0 && tid == 0;
   if (s < 0 || s >= p.num_blocks || d < 0 || d >= p.num_blocks) {
     if (first) report(p, LA_DEVERR_BLOCK_ID);
     return;
@@ -85,32 +87,40 @@ __device__ __forceinline__ void copy_part(const Params& p, long long x) {
     return;
   }
   const int units = n * p.token_units;
-  if (s == d || chunk * kChunk >= units) return;
-  uint8_t* base = p.pool[piece & 1] + (piece >> 1) * p.layer_bytes;
-  const uint8_t* from = base + s * p.block_bytes;
-  uint8_t* to = base + d * p.block_bytes;
-  // byte offset in the page of this thread's e-th unit
-  const int x0 = chunk * kChunk + tid;
-  auto at_unit = [&](int e) -> long long {
-    const int u = x0 + e * kThreads;
-    if (kFlat) return static_cast<long long>(u) * 16;
-    const int tok = u / p.token_units, r = u - tok * p.token_units;
-    const int h = r / p.row_units;
-    return tok * p.token_bytes + h * p.head_bytes + (r - h * p.row_units) * 16;
-  };
-  uint4 v[kPer];
+  if (s == d) return;
+  bool judged = false;
+  for (int part = part0; part < min(part0 + p.per, p.parts); ++part) {
+    const int piece = part / p.chunks, chunk = part - piece * p.chunks;
+    if (chunk * kChunk >= units) continue;
+    uint8_t* base = p.pool[piece & 1] + (piece >> 1) * p.layer_bytes;
+    const uint8_t* from = base + s * p.block_bytes;
+    uint8_t* to = base + d * p.block_bytes;
+    // byte offset in the page of this thread's e-th unit
+    const int x0 = chunk * kChunk + tid;
+    auto at_unit = [&](int e) -> long long {
+      const int u = x0 + e * kThreads;
+      if (kFlat) return static_cast<long long>(u) * 16;
+      const int tok = u / p.token_units, r = u - tok * p.token_units;
+      const int h = r / p.row_units;
+      return tok * p.token_bytes + h * p.head_bytes + (r - h * p.row_units) * 16;
+    };
+    uint4 v[kPer];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e)
-    if (x0 + e * kThreads < units) v[e] = __ldcs(reinterpret_cast<const uint4*>(from + at_unit(e)));
-  bool meets = false;
-  for (int j = tid; j < p.n; j += kThreads) meets |= j != i && (p.src[j] == d || (j < i && p.dst[j] == d));
-  if (__syncthreads_or(meets)) {
-    if (first) report(p, LA_DEVERR_BLOCK_PAIR);
-    return;
+    for (int e = 0; e < kPer; ++e)
+      if (x0 + e * kThreads < units) v[e] = __ldcs(reinterpret_cast<const uint4*>(from + at_unit(e)));
+    if (!judged) {
+      bool meets = false;
+      for (int j = tid; j < p.n; j += kThreads) meets |= j != i && (p.src[j] == d || (j < i && p.dst[j] == d));
+      if (__syncthreads_or(meets)) {
+        if (first) report(p, LA_DEVERR_BLOCK_PAIR);
+        return;
+      }
+      judged = true;
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (x0 + e * kThreads < units) __stcs(reinterpret_cast<uint4*>(to + at_unit(e)), v[e]);
   }
-#pragma unroll
-  for (int e = 0; e < kPer; ++e)
-    if (x0 + e * kThreads < units) __stcs(reinterpret_cast<uint4*>(to + at_unit(e)), v[e]);
 }
 
 // Entries of the table, one per thread: the first sound pair that moves the
@@ -192,13 +202,22 @@ static int setup(Params* p, void* k_pool, void* v_pool, int64_t layer_stride, in
   return LA_OK;
 }
 
+// Chunks of a pair that a CTA copies: for each 16 KB that it copies it reads at
+// most 16 KB of pairs, as long as the pair has chunks enough. (With one chunk
+// each, 16000 pages of 16 tokens in 7 layers took 9970 us, 2508 so; their bytes
+// take 2274 at the rate of a plain tensor copy.)
+static int per_cta(int pairs, int parts) { return pairs < 2048 ? 1 : pairs / 1024 < parts ? pairs / 1024 : parts; }
+
 static int launch(Params& p, cudaStream_t stream) {
   if (p.n == 0) return LA_OK;
   const int64_t entries = static_cast<int64_t>(p.table_rows) * p.table_cols;
   const int64_t table = (entries + kThreads - 1) / kThreads;
   p.chunks = (p.block_size * p.token_units + kChunk - 1) / kChunk;
-  p.pieces = 2 * p.layers;
-  const int64_t ctas = table + static_cast<int64_t>(p.n) * p.pieces * p.chunks;
+  const int64_t parts = 2 * static_cast<int64_t>(p.layers) * p.chunks;
+  if (parts > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
+  p.parts = static_cast<int>(parts);
+  p.per = per_cta(p.n, p.parts);
+  const int64_t ctas = table + (parts > 0 ? p.n * ((parts + p.per - 1) / p.per) : 0);
   if (ctas == 0) return LA_OK;
   if (ctas > 0x7fffffffLL) return LA_ERR_UNSUPPORTED;
   p.table_ctas = static_cast<int>(table);

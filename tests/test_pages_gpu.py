@@ -243,3 +243,40 @@ def test_a_table_that_names_the_pages_takes_little_beside_the_copy(pkg, cuda_dev
     to[src.long()] = dst
     assert torch.equal(table, to[names.long()])
     assert move <= 2 * copy, (move, copy)
+
+
+def test_many_pairs_in_one_call(pkg, cuda_dev):
+    """16000 pages of 16 tokens in one call take no longer than one and a half
+    times sixteen calls of 1000."""
+    n = 16000
+    k, v = (torch.zeros(4, 2 * n + n // 3, 16, 8, 128, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2))
+    src, dst, _ = _scattered(random.Random(n), k.shape[1], n, cuda_dev)
+    parts = list(zip(src.split(1000), dst.split(1000)))
+    one = _us(lambda: pkg.copy_blocks(k, v, src, dst))
+    many = _us(lambda: [pkg.copy_blocks(k, v, s, d) for s, d in parts])
+    pkg.check_device_errors(cuda_dev.index)
+    assert one <= 1.5 * many, (one, many)
+
+
+@pytest.mark.parametrize("L,bs,heads", [(1, 16, 1), (3, 16, 8), (5, 80, 3)])
+@pytest.mark.parametrize("n", [1023, 1024, 2047, 2048, 5000])
+def test_copies_of_many_pairs(pkg, cuda_dev, L, bs, heads, n):
+    """Numbers of pairs on both sides of those at which a CTA takes more of a
+    pair, with skipped pairs and counts of tokens among them."""
+    r = random.Random(n + L)
+    k, v = (_pool((L, 2 * n + 7, bs, heads, 64), torch.bfloat16, cuda_dev, s) for s in (15, 16))
+    src, dst = _ids(r, 2 * n + 7, n)
+    tokens = [r.choice((0, 1, bs // 2, bs - 1, bs)) for _ in range(n)]
+    bad = r.sample(range(n), 3)
+    dst[bad[0]], tokens[bad[1]], src[bad[2]] = -1, bs + 1, 2 * n + 7
+    done = [i for i in range(n) if i not in bad]
+    want = [_bits(x).clone() for x in (k, v)]
+    i, j, t = (torch.tensor([x[i] for i in done], device=cuda_dev) for x in (src, dst, tokens))
+    page, token = (torch.arange(bs, device=cuda_dev)[None] < t[:, None]).nonzero(as_tuple=True)
+    for w, x in zip(want, (k, v)):
+        w[:, j[page], token] = _bits(x)[:, i[page], token]
+    pkg.copy_blocks(k, v, _i32(src, cuda_dev), _i32(dst, cuda_dev), _i32(tokens, cuda_dev))
+    with pytest.raises(RuntimeError, match="outside the pool|sequence longer"):
+        pkg.check_device_errors(cuda_dev.index)
+    pkg.check_device_errors(cuda_dev.index)
+    assert torch.equal(_bits(k), want[0]) and torch.equal(_bits(v), want[1])
