@@ -125,9 +125,12 @@ __device__ __forceinline__ void copy_part(const Params& p, long long x) {
 
 // Entries of the table, one per thread: the first sound pair that moves the
 // page it names. The pairs are held in shared memory as far as they fit. A warp
-// compares its entries with one pair after another; one that some entry names is
-// judged by all its lanes together (each lane by itself, one after another,
-// 1201 pairs under 131 x 77 entries took 1.8 ms).
+// compares its entries with kLook pairs after another; a pair that some entry
+// names is judged by all its lanes together. (Each lane by itself, one after
+// another, 1201 pairs under 131 x 77 entries took 1.8 ms. One pair at a time, a
+// table that names none of them took longer than the copies beside it, 187 us,
+// since the copies' loads are in front of each look.)
+constexpr int kLook = 8;
 __device__ void table_part(const Params& p) {
   __shared__ int2 s_pair[kTablePairs];
   const int held = min(p.n, kTablePairs);
@@ -138,18 +141,28 @@ __device__ void table_part(const Params& p) {
   const long long x = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
   const bool in = x < static_cast<long long>(p.table_rows) * p.table_cols;
   int* e = in ? p.table + (x / p.table_cols) * p.table_stride + x % p.table_cols : nullptr;
-  int id = in ? *e : -1;  // -1: no entry, or one that has been replaced
-  for (int i = 0; i < p.n; ++i) {
-    const int2 m = pair(i);
-    const bool named = m.x == id && m.y != id && in_pool(p, m.x, m.y);
-    if (!__any_sync(0xffffffffu, named)) continue;
-    bool meets = false;
-    for (int j = lane; j < p.n; j += 32) {
-      const int2 o = pair(j);
-      meets |= j != i && (o.x == m.y || (j < i && o.y == m.y));
+  int id = in ? *e : -1;  // below 0: no entry, one that names no page, or one that has been replaced
+  for (int i0 = 0; i0 < p.n; i0 += kLook) {
+    bool here = false;
+    if (i0 + kLook <= held) {
+#pragma unroll
+      for (int u = 0; u < kLook; ++u) here |= s_pair[i0 + u].x == id;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLook; ++u) here |= i0 + u < p.n && p.src[i0 + u] == id;
     }
-    if (__any_sync(0xffffffffu, meets)) continue;
-    if (named) {
+    if (!__any_sync(0xffffffffu, here && id >= 0)) continue;
+    for (int i = i0; i < min(i0 + kLook, p.n); ++i) {
+      const int2 m = pair(i);
+      const bool named = m.x == id && m.y != id && in_pool(p, m.x, m.y);
+      if (!__any_sync(0xffffffffu, named)) continue;
+      bool meets = false;
+#pragma unroll 4
+      for (int j = lane; j < p.n; j += 32) {
+        const int2 o = pair(j);
+        meets |= j != i && (o.x == m.y || (j < i && o.y == m.y));
+      }
+      if (__any_sync(0xffffffffu, meets) || !named) continue;
       *e = m.y;
       id = -1;
     }
