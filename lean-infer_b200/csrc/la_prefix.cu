@@ -749,9 +749,11 @@ struct Pages {
   const int* ids_of_row;
   int boxes, per_page;  // boxes of a tile, of a page
   int win, ids, next;
+  // Not by the read-only path: the kernel in front may write the table after this
+  // one has started, and such a load need not stay behind the wait for it.
   __device__ __forceinline__ int read(const Params& p, const Segment& e, int w0, int lane) const {
     const int x = w0 * 32 + lane;
-    return x * p.box_keys < e.keys ? __ldg(ids_of_row + x / per_page) : -1;
+    return x * p.box_keys < e.keys ? __ldcg(ids_of_row + x / per_page) : -1;
   }
   __device__ __forceinline__ void start(const Params& p, const Segment& e, int lane) {
     boxes = kKeys / p.box_keys;

@@ -406,3 +406,36 @@ def test_rows_are_right_whatever_the_bounds(pkg, cuda_dev, cu, more_groups, more
     with pytest.raises(RuntimeError, match="prefix groups"):
         pkg.check_device_errors(cuda_dev.index)
     w.check(pkg, got)
+
+
+@pytest.mark.parametrize("bs", [16, 256])
+def test_decode_right_behind_a_move(pkg, cuda_dev, bs):
+    """The pages and the table that the kernel in front has just moved and
+    rewritten, to and fro, called one after another and in a graph: where a page
+    lies does not change a bit."""
+    w = Batch(cuda_dev, [(20, 1024), (5, 512)], own(28, 0, 300), bs, 16, 8, seed=21)
+    n = w.k.shape[0]
+    w.k, w.v = (torch.cat([x, torch.full_like(x, float("nan"))]) for x in (w.k, w.v))
+    r = random.Random(2)
+    here = torch.tensor(r.sample(range(1, n), (n - 1) // 2), dtype=torch.int32, device=cuda_dev)
+    there = here + n
+    first = [x.clone() for x in w.call(pkg)]
+    w.check(pkg, first)
+
+    def there_and_back():
+        got = []
+        for a, b in ((here, there), (there, here)):
+            pkg.move_blocks(w.k, w.v, a, b, w.table)
+            got.append(w.call(pkg))
+        return got
+
+    got = [x for _ in range(10) for x in there_and_back()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [x for _ in range(3) for x in there_and_back()]
+    for _ in range(5):
+        graph.replay()
+        got += [tuple(x.clone() for x in pair) for pair in captured]
+    pkg.check_device_errors(cuda_dev.index)
+    for out, lse in got:
+        assert torch.equal(out.view(torch.int16), first[0].view(torch.int16)) and torch.equal(lse, first[1])
