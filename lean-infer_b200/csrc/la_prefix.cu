@@ -1031,7 +1031,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // The plan is made before the wait for the kernel in front, from the lengths
   // and groups as they are, and checked after it; if they changed, it is made
-  // again. Beyond 256 rows or 32 groups it is made after the wait.
+  // again. Beyond 256 rows or 32 groups it is made after the wait (257 rows behind
+  // 2048 keys take 65 us, 256 of them 53).
   const bool early = p.own.batch <= 256 && p.own.groups.n <= 32;
   volatile int* stale = reinterpret_cast<volatile int*>(smem + kOffStale);
   Seen in;
