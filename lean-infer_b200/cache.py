@@ -220,16 +220,20 @@ def shared_prefix_groups(tables: Sequence[Sequence[int]], lengths: Sequence[int]
     # best[j]: blocks saved, less groups made, of the rows before cuts[j]; last[j]: where their last group begins, its prefix
     best, last = [0], [(0, 0)]
     for j in range(1, len(cuts)):
-        shared, choices = every, []
+        shared, saved = every, None
         for i in range(j - 1, -1, -1):
-            shared = min(shared, inside[i], common[cuts[i + 1]] if i + 1 < j else every)
-            if shared == 0:
+            shared, size = min(shared, inside[i]), cuts[j] - cuts[i]
+            here = best[i] + (size - 1) * shared - 1
+            if saved is None or here >= saved:
+                saved, at, prefix = here, i, shared if size > 1 else 0
+            # From further back on it shares no more than `shared`. What rows in
+            # front of cuts[i] save in it they would save, but for one row, as a
+            # group by themselves, and best[i] is no less than with that one.
+            shared = min(shared, common[cuts[i]])
+            if shared == 0 or best[i] + size * shared < saved:
                 break
-            more = cuts[j] - cuts[i] - 1
-            choices.append((best[i] + more * shared - 1, -i, shared if more else 0))
-        saved, at, prefix = max(choices)
         best.append(saved)
-        last.append((-at, prefix))
+        last.append((at, prefix))
     lens, cu, j = [], [n], len(cuts) - 1
     while cu[-1] > 0:
         j, prefix = last[j]
